@@ -13,8 +13,8 @@ from pathlib import Path
 # RPA_LIBRARY points at another build of the same library (e.g. one compiled with different tile constants).
 LIB_PATH = Path(os.environ.get("RPA_LIBRARY") or Path(__file__).resolve().parent / "lib" / "librpa_mi355x.so")
 
-RPA_ABI_VERSION = 6
-RPA_DTYPE_BF16, RPA_DTYPE_F32, RPA_DTYPE_FP8_E4M3, RPA_DTYPE_FP8_E5M2 = 0, 1, 2, 3
+RPA_ABI_VERSION = 7
+RPA_DTYPE_BF16, RPA_DTYPE_F32, RPA_DTYPE_FP8_E4M3, RPA_DTYPE_FP8_E5M2, RPA_DTYPE_INT8 = 0, 1, 2, 3, 4
 RPA_COMPUTE_BF16, RPA_COMPUTE_F32 = 0, 1
 RPA_FLAG_FORCE_GENERIC = 1
 RPA_FLAG_FP32_LOGITS = 2
@@ -38,6 +38,11 @@ EXPORTED_SYMBOLS = (
     "rpa_page_attention_launch",
     "rpa_ragged_decode_workspace_bytes",
     "rpa_ragged_decode_launch",
+    "rpa_quant_workspace_bytes",
+    "rpa_quant_fwd_launch",
+    "rpa_quant_update_launch",
+    "rpa_quant_gather_launch",
+    "rpa_block_tables_launch",
 )
 
 
@@ -150,6 +155,113 @@ class RpaRaggedDecodeParams(ctypes.Structure):
     ]
 
 
+class RpaQuantParams(ctypes.Structure):
+    """Field-for-field image of ``struct RpaQuantParams``."""
+
+    _fields_ = [
+        ("queries", ctypes.c_void_p),
+        ("kv_cache", ctypes.c_void_p),
+        ("kv_scales", ctypes.c_void_p),
+        ("context_lens", ctypes.c_void_p),
+        ("block_tables", ctypes.c_void_p),
+        ("query_start_loc", ctypes.c_void_p),
+        ("num_seqs", ctypes.c_void_p),
+        ("sinks", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+        ("query_token_stride", ctypes.c_int64),
+        ("query_head_stride", ctypes.c_int64),
+        ("total_tokens", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("scale_block", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("max_num_seqs", ctypes.c_int32),
+        ("pages_per_seq", ctypes.c_int32),
+        ("num_sinks", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+        ("logits_soft_cap", ctypes.c_float),
+        ("sliding_window", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("cache_dtype", ctypes.c_int32),
+        ("flags", ctypes.c_uint32),
+    ]
+
+
+class RpaQuantUpdateParams(ctypes.Structure):
+    """Field-for-field image of ``struct RpaQuantUpdateParams``."""
+
+    _fields_ = [
+        ("keys", ctypes.c_void_p),
+        ("values", ctypes.c_void_p),
+        ("kv_cache", ctypes.c_void_p),
+        ("kv_scales", ctypes.c_void_p),
+        ("slot_mapping", ctypes.c_void_p),
+        ("key_token_stride", ctypes.c_int64),
+        ("key_head_stride", ctypes.c_int64),
+        ("value_token_stride", ctypes.c_int64),
+        ("value_head_stride", ctypes.c_int64),
+        ("total_tokens", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("scale_block", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("cache_dtype", ctypes.c_int32),
+    ]
+
+
+class RpaQuantGatherParams(ctypes.Structure):
+    """Field-for-field image of ``struct RpaQuantGatherParams``."""
+
+    _fields_ = [
+        ("kv_cache", ctypes.c_void_p),
+        ("kv_scales", ctypes.c_void_p),
+        ("slot_mapping", ctypes.c_void_p),
+        ("keys", ctypes.c_void_p),
+        ("values", ctypes.c_void_p),
+        ("total_tokens", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("scale_block", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("cache_dtype", ctypes.c_int32),
+    ]
+
+
+class RpaBlockTablesParams(ctypes.Structure):
+    """Field-for-field image of ``struct RpaBlockTablesParams``."""
+
+    _fields_ = [
+        ("query_lens", ctypes.c_void_p),
+        ("cached_lens", ctypes.c_void_p),
+        ("block_tables", ctypes.c_void_p),
+        ("free_pages", ctypes.c_void_p),
+        ("free_state", ctypes.c_void_p),
+        ("num_seqs", ctypes.c_void_p),
+        ("query_start_loc", ctypes.c_void_p),
+        ("context_lens", ctypes.c_void_p),
+        ("slot_mapping", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("admitted", ctypes.c_void_p),
+        ("cached_lens_out", ctypes.c_void_p),
+        ("free_state_out", ctypes.c_void_p),
+        ("scratch", ctypes.c_void_p),
+        ("max_num_seqs", ctypes.c_int32),
+        ("pages_per_seq", ctypes.c_int32),
+        ("num_free_slots", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("total_tokens", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 RPA_MAX_SINK_KEYS = 64
 
 
@@ -205,6 +317,12 @@ def load() -> ctypes.CDLL:
     lib.rpa_ragged_decode_workspace_bytes.argtypes = [ctypes.POINTER(RpaRaggedDecodeParams)]
     lib.rpa_ragged_decode_launch.restype = ctypes.c_int
     lib.rpa_ragged_decode_launch.argtypes = [ctypes.POINTER(RpaRaggedDecodeParams), ctypes.c_void_p]
+    lib.rpa_quant_workspace_bytes.restype = ctypes.c_uint64
+    lib.rpa_quant_workspace_bytes.argtypes = [ctypes.POINTER(RpaQuantParams)]
+    for name, struct in (("rpa_quant_fwd_launch", RpaQuantParams), ("rpa_quant_update_launch", RpaQuantUpdateParams),
+                         ("rpa_quant_gather_launch", RpaQuantGatherParams), ("rpa_block_tables_launch", RpaBlockTablesParams)):
+        getattr(lib, name).restype = ctypes.c_int
+        getattr(lib, name).argtypes = [ctypes.POINTER(struct), ctypes.c_void_p]
     if lib.rpa_abi_version() != RPA_ABI_VERSION:
         raise NativeLibraryError(
             f"{LIB_PATH} has ABI version {lib.rpa_abi_version()}, this package expects {RPA_ABI_VERSION}: rebuild it"

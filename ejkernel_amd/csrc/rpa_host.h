@@ -104,6 +104,13 @@ int launch_tiled_fp8(const RpaParams& p, const KvLayout& kv, int kv_elem, float*
 // that run on prefill tiles, or more than kLogitStashMaxBytes).
 uint64_t logit_stash_bytes(const RpaParams& p);
 
+// The 8-bit paged cache with a scale per block of tokens and head, and the bookkeeping of a paged cache.
+int launch_quant_attention(const RpaQuantParams& p, hipStream_t stream);
+uint64_t quant_attention_workspace(const RpaQuantParams& p);
+int launch_quant_update(const RpaQuantUpdateParams& p, hipStream_t stream);
+int launch_quant_gather(const RpaQuantGatherParams& p, hipStream_t stream);
+int launch_block_tables(const RpaBlockTablesParams& p, hipStream_t stream);
+
 // Compute units of the current device (cached per device).
 int device_cu_count();
 

@@ -1,0 +1,298 @@
+// Writing to and reading from the 8-bit paged cache with a scale per block of tokens and head.
+//
+// Update.  For every run of new tokens inside one block and every combined head (K or V of a kv head):
+//   a = max |x| over the run's finite elements,  s = a / 127  or  2^ceil(log2(a / qmax)),  at least the block's old scale
+//   if the run begins inside the block;  code = round(x / s);  if s grew, the codes in front of the run are re-expressed.
+// One wavefront takes one (run, combined head): it reads the rows twice, for the maximum and for the codes (the second
+// time from the caches), and writes one byte per element, so what bounds it is the traffic of the rows, and for single
+// tokens the chain slot -> old scale -> code.  Runs are found from the slots alone: a wavefront looks at 64 tokens at once.
+#include <algorithm>
+#include <type_traits>
+
+#include "rpa_quant.h"
+
+namespace rpa {
+
+namespace {
+
+constexpr int kPiece = 8;         // elements a lane handles at once
+constexpr int kTokensPerChunk = 64;
+
+// Eight elements from `src` as floats.
+template <typename T>
+__device__ __forceinline__ void load_piece(const T* __restrict__ src, float (&x)[kPiece]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+    const uint4 w = *reinterpret_cast<const uint4*>(src);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      x[2 * k] = __uint_as_float(u[k] << 16);
+      x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+    }
+  }
+}
+
+// round(x / s) with ties to even, decided on the exact quotient.  `inv` is 1 / s rounded, so x * inv is off by three
+// roundings at most and its nearest integer q by one; r = x - q s is exact in fp32: x and q s are multiples of one unit
+// in the last place of s (or of x, where |x| < s and q is 0 or 1), and |r| < 2 s.
+__device__ __forceinline__ float round_quotient(float x, float s, float inv) {
+  float q = rintf(x * inv);
+  const float r = fmaf(-q, s, x), h = 0.5f * s;
+  const bool odd = (static_cast<int>(q) & 1) != 0;
+  if (r > h || (r == h && odd)) q += 1.f;
+  else if (r < -h || (r == -h && odd)) q -= 1.f;
+  return q;
+}
+
+// A quotient in fp64 as the fp32 number that an 8-bit floating type rounds alike: where the conversion is not exact the
+// number is moved off the middle between two codes, to the side the quotient lies on.  (Quotients of 32-bit products lie
+// on a middle or further from it than fp64 rounds.)
+__device__ __forceinline__ float off_the_middle(double v) {
+  const float f = static_cast<float>(v);
+  const double d = static_cast<double>(f);
+  if (d == v) return f;
+  return __uint_as_float(__float_as_uint(f) + (fabs(d) < fabs(v) ? 1u : ~0u));
+}
+
+// Code of x under scale s (0 where the block is all zeros).  Infinities saturate, NaN is 0.  Where the scale of a floating
+// type is a power of two, as an update makes it, x * inv is exact (or below the type's least step, too small for its
+// rounding to matter); an old scale that somebody else wrote need not be one.
+template <int kCode>
+__device__ __forceinline__ uint32_t pack4(const float* x, float s, float inv) {
+  float y[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float v = x[k];
+    v = v != v ? 0.f : v;
+    if constexpr (kCode == kCodeI8) {
+      v = s > 0.f ? (isinf(v) ? copysignf(127.f, v) : round_quotient(v, s, inv)) : 0.f;
+    } else {
+      v = !(s > 0.f) ? 0.f : (__float_as_uint(s) & 0x7fffffu) == 0 ? v * inv : off_the_middle(static_cast<double>(v) / static_cast<double>(s));
+      v = fminf(fmaxf(v, -code_max<kCode>()), code_max<kCode>());
+    }
+    y[k] = v;
+  }
+  if constexpr (kCode == kCodeI8) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w |= (static_cast<uint32_t>(static_cast<int>(y[k])) & 0xffu) << (8 * k);
+    return w;
+  } else if constexpr (kCode == kCodeE4m3) {
+    return __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false), true);
+  } else {
+    return __builtin_amdgcn_cvt_pk_bf8_f32(y[2], y[3], __builtin_amdgcn_cvt_pk_bf8_f32(y[0], y[1], 0, false), true);
+  }
+}
+
+// round(code * old / s): the codes of a word under a larger scale, in fp64, where code * old and q * s are exact products
+// of 32 bits and the quotient is too fine to be mistaken for a middle.  A code that is no number (a cache that somebody
+// else wrote) becomes 0.
+template <int kCode>
+__device__ __forceinline__ uint32_t requantize4(uint32_t w, float old, float s) {
+  if constexpr (kCode == kCodeI8) {
+    uint32_t out = 0;
+    const double ratio = static_cast<double>(old) / static_cast<double>(s), h = 0.5 * s;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const double v = static_cast<double>(code_to_f32<kCode>(w, k));
+      double q = rint(v * ratio);
+      const double r = v * old - q * s;
+      const bool odd = (static_cast<int>(q) & 1) != 0;
+      if (r > h || (r == h && odd)) q += 1.0;
+      else if (r < -h || (r == -h && odd)) q -= 1.0;
+      out |= (static_cast<uint32_t>(static_cast<int>(q)) & 0xffu) << (8 * k);
+    }
+    return out;
+  } else {
+    float y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = off_the_middle(static_cast<double>(code_to_f32<kCode>(w, k)) * old / s);
+    return pack4<kCode>(y, 1.f, 1.f);
+  }
+}
+
+// The scale a run of largest magnitude `a` asks for.
+template <int kCode>
+__device__ __forceinline__ float fresh_scale(float a) {
+  if (!(a > 0.f)) return 0.f;
+  if constexpr (kCode == kCodeI8) {
+    return fmaxf(__fdiv_rn(a, 127.f), 0x1p-126f);
+  } else {
+    // qmax = 1.75 * 2^e_max: a = m * 2^e with m in [1, 2) asks for 2^(e - e_max), doubled if m > 1.75
+    constexpr int e_max = kCode == kCodeE4m3 ? 8 : 15;
+    const uint32_t u = __float_as_uint(a);
+    const int e = static_cast<int>(u >> 23) - e_max + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return __uint_as_float(static_cast<uint32_t>(max(e, 1)) << 23);  // at least 2^-126
+  }
+}
+
+template <int kCode, typename T>
+__global__ __launch_bounds__(256) void quant_update_kernel(RpaQuantUpdateParams p, int page_shift, int block_shift) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t pool = static_cast<int64_t>(p.num_pages) << page_shift;
+  const int t = blockIdx.x * kTokensPerChunk + lane;
+  const int block_mask = (1 << block_shift) - 1;
+  // run starts among this chunk's 64 tokens
+  int slot = -1, before = -1;
+  if (t < p.total_tokens) {
+    slot = p.slot_mapping[t];
+    if (slot >= pool) slot = -1;
+    if (t > 0) before = p.slot_mapping[t - 1];
+  }
+  const bool starts = slot >= 0 && (before != slot - 1 || before < 0 || (slot & block_mask) == 0);
+  uint64_t mask = __ballot(starts);
+  const int runs = __popcll(mask), heads = 2 * p.num_kv_heads;
+  const int pieces = p.head_dim / kPiece;
+  const int workers = gridDim.y * (blockDim.x >> 6);
+  int at_run = 0;
+  for (int64_t unit = blockIdx.y * (blockDim.x >> 6) + wave; unit < static_cast<int64_t>(runs) * heads; unit += workers) {
+    const int run = static_cast<int>(unit / heads), head = static_cast<int>(unit) - run * heads;
+    for (; at_run < run; ++at_run) mask &= mask - 1;  // the runs come in order
+    const int src_lane = __ffsll(static_cast<unsigned long long>(mask)) - 1;
+    const int t0 = blockIdx.x * kTokensPerChunk + src_lane;
+    const int s0 = __builtin_amdgcn_readlane(slot, src_lane);
+    const int inside = s0 & block_mask;
+    // length of the run: consecutive slots up to the end of the block
+    int n = 1;
+    const int most = min((1 << block_shift) - inside, p.total_tokens - t0);
+    while (n < most) {
+      const int k = n + lane;
+      const bool goes_on = k < most && p.slot_mapping[t0 + k] == s0 + k;
+      const uint64_t b = __ballot(goes_on);
+      const int more = b == ~0ull ? 64 : __ffsll(static_cast<unsigned long long>(~b)) - 1;
+      n += more;
+      if (more < 64) break;
+    }
+    const int j = head >> 1;
+    const T* __restrict__ src = (head & 1) ? static_cast<const T*>(p.values) + t0 * p.value_token_stride + j * p.value_head_stride
+                                           : static_cast<const T*>(p.keys) + t0 * p.key_token_stride + j * p.key_head_stride;
+    const int64_t stride = (head & 1) ? p.value_token_stride : p.key_token_stride;
+    const int page = s0 >> page_shift, off = s0 & ((1 << page_shift) - 1);
+    const size_t row0 = ((static_cast<size_t>(page) * heads + head) << page_shift) + off;  // row of the run's first token
+    float* scale = p.kv_scales + ((static_cast<size_t>(page) * heads + head) << (page_shift - block_shift)) + (off >> block_shift);
+    const float old = inside > 0 ? *scale : 0.f;
+
+    float a = 0.f;
+    for (int e = lane; e < n * pieces; e += 64) {
+      const int row = e / pieces, piece = e - row * pieces;
+      float x[kPiece];
+      load_piece(src + row * stride + piece * kPiece, x);
+#pragma unroll
+      for (int k = 0; k < kPiece; ++k) {
+        const float m = fabsf(x[k]);
+        a = m < INFINITY ? fmaxf(a, m) : a;
+      }
+    }
+    a = wave_max(a);
+    const float want = fresh_scale<kCode>(a);
+    const float s = want > old ? want : old > 0.f ? old : want;  // an old scale that is no number counts as none
+    const float inv = s > 0.f ? 1.f / s : 0.f;
+    char* dst = static_cast<char*>(p.kv_cache) + row0 * p.head_dim;
+    for (int e = lane; e < n * pieces; e += 64) {
+      const int row = e / pieces, piece = e - row * pieces;
+      float x[kPiece];
+      load_piece(src + row * stride + piece * kPiece, x);
+      uint2 w;
+      w.x = pack4<kCode>(x, s, inv);
+      w.y = pack4<kCode>(x + 4, s, inv);
+      *reinterpret_cast<uint2*>(dst + static_cast<size_t>(e) * kPiece) = w;  // the rows of a block lie together
+    }
+    if (inside > 0 && s != old) {
+      char* head_rows = dst - static_cast<size_t>(inside) * p.head_dim;
+      const float was = old > 0.f ? old : 0.f;
+      for (int e = lane; e < inside * pieces; e += 64) {
+        uint2 w = *reinterpret_cast<const uint2*>(head_rows + static_cast<size_t>(e) * kPiece);
+        w.x = requantize4<kCode>(w.x, was, s);
+        w.y = requantize4<kCode>(w.y, was, s);
+        *reinterpret_cast<uint2*>(head_rows + static_cast<size_t>(e) * kPiece) = w;
+      }
+    }
+    if (lane == 0 && (inside == 0 || s != old)) *scale = s;
+  }
+}
+
+// Read-back: a lane takes eight elements of a row.
+template <int kCode, typename T>
+__global__ __launch_bounds__(256) void quant_gather_kernel(RpaQuantGatherParams p, int page_shift, int block_shift) {
+  const int64_t pool = static_cast<int64_t>(p.num_pages) << page_shift;
+  const int heads = 2 * p.num_kv_heads, pieces = p.head_dim / kPiece;
+  const int t = blockIdx.x;
+  const int slot = p.slot_mapping[t];
+  const bool real = slot >= 0 && slot < pool;
+  const int page = real ? slot >> page_shift : 0, off = slot & ((1 << page_shift) - 1);
+  for (int e = threadIdx.x; e < heads * pieces; e += blockDim.x) {
+    const int head = e / pieces, piece = e - head * pieces;
+    float y[kPiece];
+    if (real) {
+      const size_t line = static_cast<size_t>(page) * heads + head;
+      const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const char*>(p.kv_cache) + ((line << page_shift) + off) * p.head_dim + piece * kPiece);
+      const float s = p.kv_scales[(line << (page_shift - block_shift)) + (off >> block_shift)];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        y[k] = code_to_f32<kCode>(w.x, k) * s;
+        y[4 + k] = code_to_f32<kCode>(w.y, k) * s;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kPiece; ++k) y[k] = 0.f;
+    }
+    T* dst = static_cast<T*>((head & 1) ? p.values : p.keys) + (static_cast<size_t>(t) * p.num_kv_heads + (head >> 1)) * p.head_dim + piece * kPiece;
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float4*>(dst)[0] = make_float4(y[0], y[1], y[2], y[3]);
+      reinterpret_cast<float4*>(dst)[1] = make_float4(y[4], y[5], y[6], y[7]);
+    } else {
+      uint32_t u[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        bf16x2_t b;
+        b[0] = static_cast<__bf16>(y[2 * k]);
+        b[1] = static_cast<__bf16>(y[2 * k + 1]);
+        u[k] = __builtin_bit_cast(uint32_t, b);
+      }
+      *reinterpret_cast<uint4*>(dst) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+  }
+}
+
+template <typename F>
+void by_types(int cache_dtype, int dtype, F&& f) {
+  auto with = [&](auto code) {
+    if (dtype == RPA_DTYPE_F32) f(code, float{});
+    else f(code, bf16_t{});
+  };
+  switch (code_of_dtype(cache_dtype)) {
+    case kCodeI8: with(std::integral_constant<int, kCodeI8>{}); break;
+    case kCodeE4m3: with(std::integral_constant<int, kCodeE4m3>{}); break;
+    default: with(std::integral_constant<int, kCodeE5m2>{}); break;
+  }
+}
+
+}  // namespace
+
+int launch_quant_update(const RpaQuantUpdateParams& p, hipStream_t stream) {
+  if (p.total_tokens == 0) return RPA_OK;
+  const int chunks = (p.total_tokens + kTokensPerChunk - 1) / kTokensPerChunk;
+  // Enough wavefronts for one (run, head) each where every token is a run of its own (a decode step), and about 4096
+  // workgroups at most where the runs are longer and fewer than the tokens.
+  const int most = (2 * p.num_kv_heads * kTokensPerChunk + 3) / 4;
+  const int per_chunk = std::max(1, std::min(most, 4096 / chunks));
+  by_types(p.cache_dtype, p.dtype, [&](auto code, auto t) {
+    hipLaunchKernelGGL((quant_update_kernel<decltype(code)::value, decltype(t)>), dim3(chunks, per_chunk), dim3(256), 0, stream, p,
+                       __builtin_ctz(p.page_size), __builtin_ctz(p.scale_block));
+  });
+  return hipGetLastError() == hipSuccess ? RPA_OK : RPA_ERR_LAUNCH;
+}
+
+int launch_quant_gather(const RpaQuantGatherParams& p, hipStream_t stream) {
+  if (p.total_tokens == 0) return RPA_OK;
+  by_types(p.cache_dtype, p.dtype, [&](auto code, auto t) {
+    hipLaunchKernelGGL((quant_gather_kernel<decltype(code)::value, decltype(t)>), dim3(p.total_tokens), dim3(256), 0, stream, p,
+                       __builtin_ctz(p.page_size), __builtin_ctz(p.scale_block));
+  });
+  return hipGetLastError() == hipSuccess ? RPA_OK : RPA_ERR_LAUNCH;
+}
+
+}  // namespace rpa

@@ -3,19 +3,29 @@
 
 from .operations import (
     BaseOperationConfig,
+    BlockTables,
+    BuildBlockTables,
     FwdParams,
     PageAttention,
     PageAttentionConfig,
+    QuantizedCacheGather,
+    QuantizedCacheUpdate,
+    QuantizedRaggedPageAttention,
+    QuantizedRaggedPageAttentionConfig,
     RaggedDecodeAttention,
     RaggedDecodeAttentionConfig,
     RaggedPageAttention,
     RaggedPageAttentionConfig,
     RaggedPageAttentionv3,
     RaggedPageAttentionv3Config,
+    build_block_tables,
     page_attention,
+    quantized_cache_gather,
+    quantized_cache_update,
+    quantized_ragged_page_attention,
     ragged_decode_attention,
     ragged_page_attention,
     ragged_page_attention_v3,
 )
 
-__all__ = ['BaseOperationConfig', 'FwdParams', 'PageAttention', 'PageAttentionConfig', 'RaggedDecodeAttention', 'RaggedDecodeAttentionConfig', 'RaggedPageAttention', 'RaggedPageAttentionConfig', 'RaggedPageAttentionv3', 'RaggedPageAttentionv3Config', 'page_attention', 'ragged_decode_attention', 'ragged_page_attention', 'ragged_page_attention_v3']
+__all__ = ['BaseOperationConfig', 'BlockTables', 'BuildBlockTables', 'FwdParams', 'PageAttention', 'PageAttentionConfig', 'QuantizedCacheGather', 'QuantizedCacheUpdate', 'QuantizedRaggedPageAttention', 'QuantizedRaggedPageAttentionConfig', 'RaggedDecodeAttention', 'RaggedDecodeAttentionConfig', 'RaggedPageAttention', 'RaggedPageAttentionConfig', 'RaggedPageAttentionv3', 'RaggedPageAttentionv3Config', 'build_block_tables', 'page_attention', 'quantized_cache_gather', 'quantized_cache_update', 'quantized_ragged_page_attention', 'ragged_decode_attention', 'ragged_page_attention', 'ragged_page_attention_v3']

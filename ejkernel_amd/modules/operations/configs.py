@@ -120,3 +120,12 @@ class RaggedDecodeAttentionConfig(BaseOperationConfig):
     def validate(self) -> None:
         if self.platform not in _PLATFORMS:
             raise ValueError(f"platform={self.platform!r} must be one of {_PLATFORMS}")
+
+
+@dataclass
+class QuantizedRaggedPageAttentionConfig(BaseOperationConfig):
+    """Configuration for attention over the 8-bit cache with block scales; the work is cut on the device."""
+
+    def validate(self) -> None:
+        if self.platform not in _PLATFORMS:
+            raise ValueError(f"platform={self.platform!r} must be one of {_PLATFORMS}")

@@ -1,0 +1,145 @@
+"""Ragged paged attention over an 8-bit cache with a scale per block of tokens and head.
+
+Takes the batch of ``ragged_page_attention`` -- flat queries, context lengths, block tables, query
+starts -- and the cache of ``quantized_cache_update``.  Nothing like it is in the reference, whose
+8-bit caches have one scale per tensor and round probabilities to the cache's type: here codes are
+widened, scales enter the logits and the probabilities in float32, and only the products of
+probability and value scale are rounded, to bfloat16 (with float32 queries not even those).
+"""
+
+from __future__ import annotations
+
+import torch
+
+from ... import _native
+from .configs import QuantizedRaggedPageAttentionConfig
+from .quantized_cache import _CACHE_DTYPES, _VALUE_DTYPES, _call, _check_cache, _on_device, _rows, _strides
+from .ragged_page_attention import _call_workspace, _sinks_per_q_head
+
+__all__ = ["QuantizedRaggedPageAttention", "quantized_ragged_page_attention"]
+
+
+class QuantizedRaggedPageAttention:
+    """Kernel object of ``quantized_ragged_page_attention``."""
+
+    op_id = "quantized_ragged_page_attention"
+
+    def run(self, queries, kv_cache, kv_scales, context_lens, block_tables, query_start_loc, num_seqs, softmax_aux=None, *,
+            softmax_scale: float | None = None, logits_soft_cap: float | None = None, sliding_window: int | None = None,
+            cfg: QuantizedRaggedPageAttentionConfig):
+        cfg.validate()
+        block = _check_cache(kv_cache, kv_scales)
+        num_pages, heads, page_size, head_dim = kv_cache.shape
+        num_kv_heads = heads // 2
+        if queries.dim() != 3 or queries.shape[2] != head_dim:
+            raise ValueError(f"queries must be [total_tokens, num_q_heads, {head_dim}], got {tuple(queries.shape)}")
+        if queries.dtype not in _VALUE_DTYPES:
+            raise ValueError(f"queries.dtype={queries.dtype} must be bfloat16 or float32")
+        total_tokens, num_q_heads, _ = queries.shape
+        if num_q_heads == 0 or num_q_heads % num_kv_heads != 0:
+            raise ValueError(f"{num_q_heads=} must be divisible by {num_kv_heads=}")
+        if block_tables.dim() != 2 or 0 in block_tables.shape:
+            raise ValueError(f"block_tables must be [max_num_seqs, pages_per_seq], got {tuple(block_tables.shape)}")
+        max_num_seqs, pages_per_seq = block_tables.shape
+        if tuple(context_lens.shape) != (max_num_seqs,):
+            raise ValueError(f"context_lens.shape={tuple(context_lens.shape)} must be ({max_num_seqs},)")
+        if tuple(query_start_loc.shape) != (max_num_seqs + 1,):
+            raise ValueError(f"query_start_loc.shape={tuple(query_start_loc.shape)} must be ({max_num_seqs + 1},)")
+        if not isinstance(num_seqs, torch.Tensor):
+            num_seqs = torch.tensor([int(num_seqs)], dtype=torch.int32, device=queries.device)
+        elif tuple(num_seqs.shape) != (1,):
+            raise ValueError(f"num_seqs.shape={tuple(num_seqs.shape)} must be (1,)")
+        for name, t in (("context_lens", context_lens), ("block_tables", block_tables), ("query_start_loc", query_start_loc),
+                        ("num_seqs", num_seqs)):
+            if t.dtype != torch.int32:
+                raise ValueError(f"{name}.dtype={t.dtype} must be int32")
+        if sliding_window is not None and sliding_window <= 0:
+            raise ValueError(f"{sliding_window=} must be positive.")
+        if logits_soft_cap is not None and logits_soft_cap == 0.0:
+            raise ValueError(f"{logits_soft_cap=} must not be 0.0.")
+        if any(t.requires_grad for t in (queries, kv_scales)):
+            raise NotImplementedError("quantized_ragged_page_attention is forward-only; detach the inputs")
+        dev = _on_device("quantized_ragged_page_attention", queries, kv_cache=kv_cache, kv_scales=kv_scales, context_lens=context_lens,
+                         block_tables=block_tables, query_start_loc=query_start_loc, num_seqs=num_seqs)
+        out = torch.empty(queries.shape, dtype=queries.dtype, device=dev)
+        if total_tokens == 0:
+            return out
+        queries = _rows(queries)
+        context_lens, block_tables, query_start_loc = context_lens.contiguous(), block_tables.contiguous(), query_start_loc.contiguous()
+        p = _native.RpaQuantParams()
+        if softmax_aux is not None and softmax_aux.shape[-1] > 0:
+            sinks = _sinks_per_q_head(softmax_aux.to(dev), num_q_heads, num_kv_heads)
+            p.sinks, p.num_sinks = sinks.data_ptr(), sinks.shape[1]
+        p.queries, p.kv_cache, p.kv_scales = queries.data_ptr(), kv_cache.data_ptr(), kv_scales.data_ptr()
+        p.context_lens, p.block_tables = context_lens.data_ptr(), block_tables.data_ptr()
+        p.query_start_loc, p.num_seqs, p.out = query_start_loc.data_ptr(), num_seqs.data_ptr(), out.data_ptr()
+        p.query_token_stride, p.query_head_stride = _strides(queries)
+        p.total_tokens, p.num_q_heads, p.num_kv_heads, p.head_dim = total_tokens, num_q_heads, num_kv_heads, head_dim
+        p.page_size, p.scale_block, p.num_pages = page_size, block, num_pages
+        p.max_num_seqs, p.pages_per_seq = max_num_seqs, pages_per_seq
+        p.softmax_scale = head_dim**-0.5 if softmax_scale is None else softmax_scale
+        p.logits_soft_cap = 0.0 if logits_soft_cap is None else logits_soft_cap
+        p.sliding_window = 0 if sliding_window is None else min(sliding_window, 2**31 - 1)
+        p.dtype, p.cache_dtype = _VALUE_DTYPES[queries.dtype], _CACHE_DTYPES[kv_cache.dtype]
+        workspace = _call_workspace(dev, p, "rpa_quant_workspace_bytes")
+        p.workspace, p.workspace_bytes = workspace.data_ptr(), workspace.numel()
+        _call("rpa_quant_fwd_launch", p, dev)
+        return out
+
+    def heuristic_cfg(self, inv=None) -> QuantizedRaggedPageAttentionConfig:
+        """The work is cut on the device; there is nothing to choose."""
+        return QuantizedRaggedPageAttentionConfig()
+
+    def candidate_cfgs(self, inv=None) -> list[QuantizedRaggedPageAttentionConfig]:
+        """One implementation, one candidate."""
+        return [self.heuristic_cfg(inv)]
+
+    def __call__(self, *args, **kwargs):
+        kwargs.setdefault("cfg", self.heuristic_cfg())
+        return self.run(*args, **kwargs)
+
+
+_kernel = QuantizedRaggedPageAttention()
+_default_cfg = QuantizedRaggedPageAttentionConfig()
+
+
+def quantized_ragged_page_attention(
+    queries,
+    kv_cache,
+    kv_scales,
+    context_lens,
+    block_tables,
+    query_start_loc,
+    num_seqs,
+    softmax_aux=None,
+    /,
+    *,
+    softmax_scale: float | None = None,
+    logits_soft_cap: float | None = None,
+    sliding_window: int | None = None,
+    cfg: QuantizedRaggedPageAttentionConfig | None = None,
+):
+    """Attention of a mixed prefill + decode batch over the 8-bit paged cache.
+
+    Args:
+        queries: ``[total_tokens, num_q_heads, head_dim]`` bfloat16 or float32, all sequences one after another;
+            views with strides of whole 16-byte pieces are read in place.
+        kv_cache: ``[num_pages, 2 * num_kv_heads, page_size, head_dim]`` int8, float8_e4m3fn or float8_e5m2;
+            K of kv head ``j`` at ``2j``, V at ``2j + 1``.  Every value a sequence can see must be finite.
+        kv_scales: ``[num_pages, 2 * num_kv_heads, page_size // block]`` float32.
+        context_lens: ``[max_num_seqs]`` int32, keys of each sequence including its query tokens.
+        block_tables: ``[max_num_seqs, pages_per_seq]`` int32; entries behind a sequence's pages are not read.
+        query_start_loc: ``[max_num_seqs + 1]`` int32 cumulative query lengths.
+        num_seqs: ``[1]`` int32 tensor (or int), sequences present.
+        softmax_aux: optional sink logits ``[num_kv_heads | num_q_heads, n_sinks]`` or ``[n_sinks]``.
+        softmax_scale: defaults to ``head_dim ** -0.5``.
+        logits_soft_cap: ``cap * tanh(logits / cap)`` before masking.
+        sliding_window: keep keys with ``k_pos > q_pos - window``.
+
+    Returns:
+        ``[total_tokens, num_q_heads, head_dim]`` in the dtype of ``queries``; rows without a visible key and rows
+        at or beyond ``query_start_loc[num_seqs]`` are zero.
+    """
+    return _kernel.run(queries, kv_cache, kv_scales, context_lens, block_tables, query_start_loc, num_seqs, softmax_aux,
+                       softmax_scale=softmax_scale, logits_soft_cap=logits_soft_cap, sliding_window=sliding_window,
+                       cfg=_default_cfg if cfg is None else cfg)

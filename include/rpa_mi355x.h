@@ -25,13 +25,15 @@
 extern "C" {
 #endif
 
-#define RPA_ABI_VERSION 6
+#define RPA_ABI_VERSION 7
 
 /* element type of queries / kv_pages / out */
 #define RPA_DTYPE_BF16 0
 #define RPA_DTYPE_F32 1
 #define RPA_DTYPE_FP8_E4M3 2 /* OCP e4m3 (finite, no infinities; jnp.float8_e4m3fn): cache of rpa_v3_launch only */
 #define RPA_DTYPE_FP8_E5M2 3 /* OCP e5m2 (jnp.float8_e5m2): cache of rpa_v3_launch only */
+
+#define RPA_DTYPE_INT8 4     /* symmetric int8 codes -127..127: cache of the rpa_quant_* entry points only              */
 
 /* arithmetic mode */
 #define RPA_COMPUTE_BF16 0 /* bf16 MFMA contractions, fp32 online softmax, reference rounding points */
@@ -277,6 +279,136 @@ typedef struct RpaRaggedDecodeParams {
 
 uint64_t rpa_ragged_decode_workspace_bytes(const RpaRaggedDecodeParams* dims);
 int rpa_ragged_decode_launch(const RpaRaggedDecodeParams* params, void* hip_stream);
+
+/*
+ * The 8-bit paged cache with a scale per block of tokens and head, and what works on it (no counterpart in the
+ * reference, whose 8-bit caches have one scale per tensor).
+ *
+ *   kv_cache  [num_pages, 2*num_kv_heads, page_size, head_dim] codes, int8 / e4m3 / e5m2; K of kv head j at 2j, V at
+ *             2j + 1.  The tokens of a page lie together for each head, so the block one scale covers is contiguous.
+ *   kv_scales [num_pages, 2*num_kv_heads, page_size / scale_block] fp32; element = code * scale of its block.
+ *
+ * head_dim is a multiple of 16 from 16 to 256, page_size a power of two from 4 to 32768, scale_block a power of two from 4
+ * to page_size, num_pages * page_size below 2^31.  Slot = page * page_size + offset names a token's place in the pool.
+ */
+
+/* Attention over that cache: queries of every sequence against its keys, causal from the end of its context, with the
+ * window, soft cap and sinks of rpa_fwd_launch.  Logits, softmax and sums are fp32; with bf16 queries the probabilities
+ * times the value scale are rounded to bf16 for the matrix unit, with fp32 queries nothing is rounded below fp32.
+ * Rows without a visible key, and rows at or beyond query_start_loc[num_seqs], are zeros. */
+typedef struct RpaQuantParams {
+  const void* queries;            /* [total_tokens, num_q_heads, head_dim] bf16 or fp32, strides below; 16-byte aligned */
+  const void* kv_cache;           /* 16-byte aligned                                                                   */
+  const float* kv_scales;
+  const int32_t* context_lens;    /* [max_num_seqs] keys of each sequence, its query tokens included                   */
+  const int32_t* block_tables;    /* [max_num_seqs, pages_per_seq]                                                     */
+  const int32_t* query_start_loc; /* [max_num_seqs + 1]                                                                */
+  const int32_t* num_seqs;        /* [1]                                                                               */
+  const float* sinks;             /* [num_q_heads, num_sinks] or NULL                                                  */
+  void* out;                      /* [total_tokens, num_q_heads, head_dim], dtype of the queries                       */
+  void* workspace;                /* >= rpa_quant_workspace_bytes() bytes, cleared once with rpa_workspace_init        */
+  uint64_t workspace_bytes;
+  int64_t query_token_stride;     /* elements between the tokens and between the heads of `queries`; multiples of 16   */
+  int64_t query_head_stride;      /* bytes                                                                             */
+  int32_t total_tokens;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t page_size;
+  int32_t scale_block;
+  int32_t num_pages;
+  int32_t max_num_seqs;
+  int32_t pages_per_seq;
+  int32_t num_sinks;
+  float softmax_scale;
+  float logits_soft_cap;          /* 0 = none */
+  int32_t sliding_window;         /* 0 = none */
+  int32_t dtype;                  /* RPA_DTYPE_BF16 or RPA_DTYPE_F32                            */
+  int32_t cache_dtype;            /* RPA_DTYPE_INT8, RPA_DTYPE_FP8_E4M3 or RPA_DTYPE_FP8_E5M2   */
+  uint32_t flags;                 /* 0 */
+} RpaQuantParams;
+uint64_t rpa_quant_workspace_bytes(const RpaQuantParams* dims);
+int rpa_quant_fwd_launch(const RpaQuantParams* params, void* hip_stream);
+
+/* Writes the rows of new tokens into the cache.  Token t goes to slot_mapping[t]; a slot outside the pool (-1) skips it.
+ * Consecutive tokens in consecutive slots of one block are a run, written with one scale per head:
+ *   a = largest finite |x| of the run; s = a / 127 (int8) or the least power of two with a <= qmax * s (fp8), at least
+ *   2^-126, 0 if a is 0.  A run that begins inside a block keeps the rows before it: s is then at least the block's old
+ *   scale, and if it is larger the codes of those rows become round(code * old / s).
+ * Codes are round(x / s), ties to even, decided on the exact quotient; infinities become the largest code, NaN 0.
+ * The rows behind a run are stale.  A block written by two runs of one call ends with either's scale. */
+typedef struct RpaQuantUpdateParams {
+  const void* keys;               /* [total_tokens, num_kv_heads, head_dim] bf16 or fp32, 16-byte aligned */
+  const void* values;
+  void* kv_cache;
+  float* kv_scales;
+  const int32_t* slot_mapping;    /* [total_tokens] */
+  int64_t key_token_stride;       /* elements between tokens and heads; multiples of 16 bytes */
+  int64_t key_head_stride;
+  int64_t value_token_stride;
+  int64_t value_head_stride;
+  int32_t total_tokens;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t page_size;
+  int32_t scale_block;
+  int32_t num_pages;
+  int32_t dtype;
+  int32_t cache_dtype;
+} RpaQuantUpdateParams;
+int rpa_quant_update_launch(const RpaQuantUpdateParams* params, void* hip_stream);
+
+/* Reads rows back as values: keys / values [total_tokens, num_kv_heads, head_dim] (contiguous, 16-byte aligned) of the
+ * slots in slot_mapping: code * scale in fp32, rounded to `dtype`; a slot outside the pool gives a row of zeros. */
+typedef struct RpaQuantGatherParams {
+  const void* kv_cache;
+  const float* kv_scales;
+  const int32_t* slot_mapping;
+  void* keys;
+  void* values;
+  int32_t total_tokens;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t page_size;
+  int32_t scale_block;
+  int32_t num_pages;
+  int32_t dtype;
+  int32_t cache_dtype;
+} RpaQuantGatherParams;
+int rpa_quant_gather_launch(const RpaQuantGatherParams* params, void* hip_stream);
+
+/* One step of the bookkeeping of a paged cache, on the device.  The free pages are a ring: free_pages[(head + i) %
+ * num_free_slots] for i < count, with free_state = {head, count}.  For s < num_seqs, in order:
+ *   query_lens[s] > 0   the request gets the pages its new tokens need beyond ceil(cached_lens[s] / page_size).  It is
+ *                       refused (admitted[s] = 0, nothing taken) if its context would pass pages_per_seq pages, if its
+ *                       tokens end behind total_tokens, or if it needs pages and the needs up to its own exceed the ring.
+ *   query_lens[s] == 0  it idles: nothing changes.
+ *   query_lens[s] < 0   it has ended: its pages go back to the ring (behind the free ones, in the order of its table).
+ * block_tables and free_pages are updated in place; entries of a table behind a request's pages keep what they hold.
+ * Page ids are taken as they stand.  Sequences from num_seqs on have no tokens, a context of 0 and keep their cached_lens. */
+typedef struct RpaBlockTablesParams {
+  const int32_t* query_lens;      /* [max_num_seqs] */
+  const int32_t* cached_lens;     /* [max_num_seqs] tokens in the cache before this step */
+  int32_t* block_tables;          /* [max_num_seqs, pages_per_seq] */
+  int32_t* free_pages;            /* [num_free_slots] */
+  const int32_t* free_state;      /* [2] head, count */
+  const int32_t* num_seqs;        /* [1] */
+  int32_t* query_start_loc;       /* [max_num_seqs + 1] prefix sums of the query lengths, at most total_tokens */
+  int32_t* context_lens;          /* [max_num_seqs] cached + new tokens; 0 for refused and ended requests */
+  int32_t* slot_mapping;          /* [total_tokens] -1 for tokens of refused requests and rows behind the last token */
+  int32_t* positions;             /* [total_tokens] position in the sequence, -1 as above */
+  int32_t* admitted;              /* [max_num_seqs] 1: the request's tokens run (or it idles); 0: refused or ended */
+  int32_t* cached_lens_out;       /* [max_num_seqs] cached_lens of the next step; 0 for ended requests */
+  int32_t* free_state_out;        /* [2] */
+  int32_t* scratch;               /* [4 * max_num_seqs + 4] int32 */
+  int32_t max_num_seqs;
+  int32_t pages_per_seq;
+  int32_t num_free_slots;
+  int32_t page_size;
+  int32_t total_tokens;
+  int32_t reserved;               /* 0 */
+} RpaBlockTablesParams;
+int rpa_block_tables_launch(const RpaBlockTablesParams* params, void* hip_stream);
 
 /* Message for the calling thread's most recent failure ("" if none). */
 const char* rpa_last_error(void);
