@@ -20,7 +20,8 @@ LIB_DIR = PKG_DIR / "lib"
 LIB_PATH = LIB_DIR / "librpa_mi355x.so"
 OBJ_DIR = PKG_DIR / "build"
 
-SOURCES = ["rpa_tile.hip", "rpa_quant_attn.hip", "rpa_api.hip", "rpa_block_tables.hip", "rpa_generic.hip", "rpa_kv_update.hip",
+SOURCES = ["rpa_tile.hip", "rpa_quant_attn_i8.hip", "rpa_quant_attn_e4m3.hip", "rpa_quant_attn_e5m2.hip",
+           "rpa_quant_attn.hip", "rpa_api.hip", "rpa_block_tables.hip", "rpa_generic.hip", "rpa_kv_update.hip",
            "rpa_quant_api.hip", "rpa_quant_cache.hip", "rpa_sink_keys.hip"]
 # -packed-fp32-ops is switched off on purpose: the compiler must not form v_pk_*_f32.
 HIPCC_FLAGS = [
@@ -51,7 +52,7 @@ def _compile(src: str, extra: list[str]) -> Path:
     return obj
 
 
-def build(verbose: bool = True, extra_flags: list[str] | None = None, jobs: int = 4) -> Path:
+def build(verbose: bool = True, extra_flags: list[str] | None = None, jobs: int = 8) -> Path:
     """Compile all sources and link the shared library. Always recompiles."""
     extra = list(extra_flags or [])
     OBJ_DIR.mkdir(exist_ok=True)

@@ -6,10 +6,10 @@
 
 #include "rpa_device.h"
 #include "rpa_host.h"
+#include "rpa_tile_common.h"
 
 namespace rpa {
 
-typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
 
 // Types of the codes.
 constexpr int kCodeI8 = 0, kCodeE4m3 = 1, kCodeE5m2 = 2;

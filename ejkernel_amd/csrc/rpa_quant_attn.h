@@ -1,0 +1,1012 @@
+// Attention over the 8-bit paged cache with a scale per block of tokens and head: the kernel.
+//
+//   out[row] = sum_k p_k v_k vs_k / (sum_k p_k + sum_j e^(sink_j)),  p_k = exp(cap(scale q . k_k ks_k))
+//
+// Codes are widened to bf16, which holds all of them exactly, and multiplied on the matrix units; the scale of a key
+// enters its logit and the scale of a value its probability, in fp32.  With bf16 queries p vs is rounded to bf16 once;
+// with fp32 queries the operands that have 24 bits -- q and p vs -- are split into three bf16 parts each (8 + 8 + 8 bits),
+// three products in place of one, and nothing is rounded below fp32.
+//
+// One launch of 2 workgroups per compute unit.  The batch is two streams of keys.  A sequence with at most 16 query rows
+// per kv head (a decode step) is one item per kv head of the first stream: its rows fill one 16-wide matrix tile, and the
+// four wavefronts of a workgroup take every fourth tile of 32 keys and meet in LDS at its end; nothing is shared between
+// them on the way, so they load straight into registers.  What bounds this stream is memory.  Other sequences are cut into
+// tiles of rows, an item each of the second stream: the workgroup widens 8 KiB of K and of V codes at a time into LDS, in
+// the order in which the matrix unit takes them, and each wavefront multiplies them with its own rows.  What bounds it is
+// matrix, LDS and exp throughput.  Each stream is cut into equal runs of keys, one per workgroup, wherever the cut falls:
+// few long sequences, one long chunk and a ragged batch all fill the device.  An item that is cut leaves its parts'
+// (maximum, sum, output) in the workspace, and the workgroup that hands in the last part adds them up in stream order,
+// so that results do not depend on who that is.  Half of the workgroups take their run of the second stream first, so that
+// one workgroup of a compute unit waits for memory while the other multiplies.
+#pragma once
+
+#include "rpa_quant.h"
+#include "rpa_tile_common.h"
+
+namespace rpa {
+
+struct QuantArgs {
+  RpaQuantParams p;
+  int page_shift, block_shift;
+  int group;        // query heads per kv head
+  int tile_group;   // rows of one token in a tile of the second stream: min(group, rows of a tile)
+  int tile_tokens;  // tokens of a tile
+  int subs;         // tiles side by side for the heads of one token, where they are more than a tile's rows
+  int grid;         // workgroups, a multiple of 8
+  uint32_t* tickets;        // [2 * grid], zero between launches
+  float* thin_o;            // [2 * grid][16 * D] states of cut items of the first stream, as they lie in registers
+  float* thin_ml;           // [2 * grid][16][2]
+  float* tile_o;            // [2 * grid][rows * D]
+  float* tile_ml;           // [2 * grid][rows][2]
+};
+
+// Shape of the second stream's tiles for a (padded) head_dim: keys per step, and 16-row tiles per wavefront.
+template <int D>
+constexpr int quant_step_keys() { return 8192 / D; }
+template <int D, int kParts>
+constexpr int quant_row_tiles() { return kParts == 3 ? 1 : 2; }
+
+constexpr int kThinStep = 128;     // keys a workgroup takes at once in the first stream
+constexpr int kThinPad = 128;      // what an item of the first stream costs beyond its keys, in keys
+constexpr int kTilePad = 64;       // the same of the second
+constexpr int kThinLeast = 256;    // least run of keys per workgroup
+constexpr int kTileLeast = 512;
+constexpr float kNoKey = -3.0e38f; // row maximum before any key
+constexpr float kLazy = 8.f;       // the running maximum follows when a logit passes it by 2^8
+constexpr int kAgentScope = 16;    // auxiliary bit of a buffer access: coherent across the device's L2s
+
+namespace quant {
+
+struct Seq {
+  int q0, q_len, kv_len;
+};
+
+__device__ __forceinline__ int64_t ramp(int64_t n, int64_t c, int64_t d) {  // sum over i < n of max(0, c + i d)
+  const int64_t i0 = c >= 0 ? 0 : (d - 1 - c) / d;
+  const int64_t m = n > i0 ? n - i0 : 0;
+  return m * (c + i0 * d) + d * (m * (m - 1) / 2);
+}
+
+// Keys of the rows of tokens [t0, t1) of a sequence: [first, end).
+struct Range {
+  int first, end;
+};
+__device__ __forceinline__ Range key_range(const QuantArgs& a, const Seq& q, int t0, int t1) {
+  const int base = q.kv_len - q.q_len;
+  Range r;
+  r.end = max(base + t1, 0);
+  const int64_t f = static_cast<int64_t>(base) + t0 - a.p.sliding_window + 1;
+  r.first = a.p.sliding_window > 0 && f > 0 ? static_cast<int>(f) : 0;
+  return r;
+}
+
+// The second stream: tiles of one (sequence, head).
+__device__ __forceinline__ int tiles_of(const QuantArgs& a, const Seq& q) { return (q.q_len + a.tile_tokens - 1) / a.tile_tokens; }
+// Stream positions in front of tile n (n below the number of tiles), or of all tiles.
+__device__ __forceinline__ int64_t tiles_before(const QuantArgs& a, const Seq& q, int n, bool all) {
+  const int64_t base = q.kv_len - q.q_len, d = a.tile_tokens;
+  int64_t sum = ramp(n, base + d, d) + static_cast<int64_t>(n) * kTilePad;
+  if (a.p.sliding_window > 0) sum -= ramp(n, base - a.p.sliding_window + 1, d);
+  if (all) sum -= max(base + n * d, static_cast<int64_t>(0)) - max(base + q.q_len, 0);
+  return sum;
+}
+
+__device__ __forceinline__ bool is_thin(const QuantArgs& a, const Seq& q) { return static_cast<int64_t>(q.q_len) * a.group <= 16; }
+
+__device__ __forceinline__ int thin_keys(const QuantArgs& a, const Seq& q) {
+  const Range r = key_range(a, q, 0, q.q_len);
+  return r.end - r.first;
+}
+
+__device__ __forceinline__ Seq load_seq(const QuantArgs& a, int n, int s) {
+  Seq q = {0, 0, 0};
+  if (s < n) {
+    q.q0 = min(max(a.p.query_start_loc[s], 0), a.p.total_tokens);
+    q.q_len = max(min(max(a.p.query_start_loc[s + 1], 0), a.p.total_tokens) - q.q0, 0);
+    const int64_t room = static_cast<int64_t>(a.p.pages_per_seq) << a.page_shift;
+    q.kv_len = static_cast<int>(min(static_cast<int64_t>(max(a.p.context_lens[s], 0)), room));
+  }
+  return q;
+}
+
+// A cut of a stream of `total` positions over `n` workgroups: run w is [bound(w), bound(w + 1)).
+struct Cut {
+  int64_t total;
+  int n;
+  __device__ __forceinline__ int64_t bound(int w) const { return total * w / n; }
+  __device__ __forceinline__ int owner(int64_t x) const { return static_cast<int>(((x + 1) * n - 1) / total); }
+};
+
+// Lengths of 64 sequences at a time, a lane each.
+struct Window {
+  Seq mine;
+  int base = -1;
+  __device__ __forceinline__ void at(const QuantArgs& a, int n, int s) {
+    if (base >= 0 && s >= base && s < base + 64) return;
+    base = s;
+    mine = load_seq(a, n, s + (threadIdx.x & 63));
+  }
+  __device__ __forceinline__ Seq get(int s) const {
+    const int l = s - base;
+    return {__builtin_amdgcn_readlane(mine.q0, l), __builtin_amdgcn_readlane(mine.q_len, l), __builtin_amdgcn_readlane(mine.kv_len, l)};
+  }
+  // The first sequence from s on that is in the stream, or n.
+  __device__ __forceinline__ int next(const QuantArgs& a, int n, int s, bool thin) {
+    while (s < n) {
+      at(a, n, s);
+      const uint64_t m = __ballot(mine.q_len > 0 && is_thin(a, mine) == thin) >> (s - base);
+      if (m != 0) return s + __ffsll(static_cast<unsigned long long>(m)) - 1;
+      s = base + 64;
+    }
+    return n;
+  }
+};
+
+// First key row of (page of key k, combined head) in the pool, in rows of the head's page.
+__device__ __forceinline__ int page_of_key(const QuantArgs& a, const int32_t* __restrict__ table, int k, int last_page) {
+  return clamp_page(table[min(k >> a.page_shift, last_page)], a.p.num_pages);
+}
+__device__ __forceinline__ const char* row_of(const QuantArgs& a, int page, int head, int k) {
+  const uint64_t line = static_cast<uint64_t>(page) * (2 * a.p.num_kv_heads) + head;
+  const uint64_t row = (line << a.page_shift) + (k & ((1 << a.page_shift) - 1));
+  return static_cast<const char*>(a.p.kv_cache) + row * a.p.head_dim;
+}
+__device__ __forceinline__ const float* scale_of(const QuantArgs& a, int page, int head, int k) {
+  const uint64_t line = static_cast<uint64_t>(page) * (2 * a.p.num_kv_heads) + head;
+  return a.p.kv_scales + (line << (a.page_shift - a.block_shift)) + ((k & ((1 << a.page_shift) - 1)) >> a.block_shift);
+}
+
+// bf16 parts of eight fp32 values: part 0 is the value rounded, part 1 the rest of it rounded, part 2 the rest of that.
+template <int kParts>
+__device__ __forceinline__ void split(const float (&x)[8], bf16x8_t (&part)[kParts]) {
+  float r[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = x[e];
+#pragma unroll
+  for (int s = 0; s < kParts; ++s) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      part[s][e] = static_cast<__bf16>(r[e]);
+      if (s + 1 < kParts) r[e] -= static_cast<float>(part[s][e]);
+    }
+  }
+}
+
+// Eight query elements from element d of a row (zeros where the row or the element does not exist).
+template <typename T, int kParts>
+__device__ __forceinline__ void load_q(const T* row, bool real, int d, int head_dim, bf16x8_t (&part)[kParts]) {
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if constexpr (sizeof(T) == 2) {
+    u32x4_t w = {0u, 0u, 0u, 0u};
+    if (real && d < head_dim) w = *reinterpret_cast<const u32x4_t*>(row + d);
+    part[0] = __builtin_bit_cast(bf16x8_t, w);
+  } else {
+    if (real && d < head_dim) {
+      const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(row + d), hi = *reinterpret_cast<const f32x4_t*>(row + d + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = lo[e], x[4 + e] = hi[e];
+    }
+    split<kParts>(x, part);
+  }
+}
+
+// 16 codes -> two operands of eight bf16.
+template <int kCode>
+__device__ __forceinline__ void widen16(u32x4_t w, bf16x8_t (&op)[2]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    u32x4_t o;
+    o[0] = codes_to_bf16<kCode, false>(w[2 * h]);
+    o[1] = codes_to_bf16<kCode, true>(w[2 * h]);
+    o[2] = codes_to_bf16<kCode, false>(w[2 * h + 1]);
+    o[3] = codes_to_bf16<kCode, true>(w[2 * h + 1]);
+    op[h] = __builtin_bit_cast(bf16x8_t, o);
+  }
+}
+
+// Byte b of two words (two keys) as a pair of bf16, for all four bytes.
+template <int kCode>
+__device__ __forceinline__ void widen_pairs(uint32_t x, uint32_t y, uint32_t (&pair)[4]) {
+  if constexpr (kCode == kCodeI8) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const float f = static_cast<float>(static_cast<int8_t>(x >> (8 * b))), g = static_cast<float>(static_cast<int8_t>(y >> (8 * b)));
+      pair[b] = __builtin_amdgcn_perm(__float_as_uint(g), __float_as_uint(f), 0x07060302u);
+    }
+  } else {
+    const uint32_t lo = __builtin_amdgcn_perm(y, x, 0x05010400u), hi = __builtin_amdgcn_perm(y, x, 0x07030602u);
+    pair[0] = codes_to_bf16<kCode, false>(lo);
+    pair[1] = codes_to_bf16<kCode, true>(lo);
+    pair[2] = codes_to_bf16<kCode, false>(hi);
+    pair[3] = codes_to_bf16<kCode, true>(hi);
+  }
+}
+
+__device__ __forceinline__ f32x4_t mfma(bf16x8_t a, bf16x8_t b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// Eight logits of a row (keys k0 + 4 g + r and k0 + 16 + 4 g + r of the lane's group g) in units of log2, masked to
+// [lo, hi) where `edge`.
+struct Logits {
+  float x[2][4];
+};
+template <bool kCap>
+__device__ __forceinline__ float scaled(float s, float c, float cap, float inv_cap) {
+  if constexpr (kCap) return cap * tanh_fast(s * c * inv_cap);
+  return s * c;
+}
+
+// Adds the row's sinks to its sum: (m, l) -> weight of the output and sum under the larger of the two maxima.
+__device__ __forceinline__ void add_sinks(const QuantArgs& a, int head, float m, float& l, float& weight) {
+  weight = 1.f;
+  if (a.p.num_sinks == 0 || !(l > 0.f)) return;
+  const float* sink = a.p.sinks + static_cast<size_t>(head) * a.p.num_sinks;
+  float top = m;
+  for (int j = 0; j < a.p.num_sinks; ++j) top = fmaxf(top, sink[j] * kLog2e);
+  weight = __builtin_amdgcn_exp2f(m - top);
+  l *= weight;
+  for (int j = 0; j < a.p.num_sinks; ++j) l += __builtin_amdgcn_exp2f(sink[j] * kLog2e - top);
+}
+
+// N fp32 results to the output, N a multiple of 4.
+template <typename T, int N>
+__device__ __forceinline__ void store_row(T* dst, const float (&o)[N]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int k = 0; k < N / 4; ++k) *reinterpret_cast<f32x4_t*>(dst + 4 * k) = f32x4_t{o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]};
+  } else {
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) w[k] = pack_bf16x2(o[2 * k], o[2 * k + 1]);
+    if constexpr (N % 8 == 0) {
+#pragma unroll
+      for (int k = 0; k < N / 8; ++k) *reinterpret_cast<u32x4_t*>(dst + 8 * k) = u32x4_t{w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]};
+    } else {
+      *reinterpret_cast<u32x2_t*>(dst) = u32x2_t{w[0], w[1]};
+    }
+  }
+}
+
+// Who else holds parts of an item that starts at stream position x0 and has `keys` keys (`step` of them at once).
+struct Parts {
+  int first, count;  // workgroup of the first part, number of parts
+  bool head;         // the first part begins the item (else the workgroup where the item starts has none of its keys)
+};
+__device__ __forceinline__ Parts parts_of(const Cut& cut, int64_t x0, int keys, int step) {
+  Parts r;
+  const int w0 = cut.owner(x0), w1 = cut.owner(x0 + keys - 1);
+  r.head = w1 == w0 || cut.bound(w0 + 1) - x0 >= step;
+  r.first = r.head ? w0 : w0 + 1;
+  r.count = w1 - r.first + 1;
+  return r;
+}
+// A part's place in the workspace: the run's first item (begun by an earlier workgroup) or its last.
+__device__ __forceinline__ int slot_of(const Parts& parts, int k) { return 2 * (parts.first + k) + (parts.head && k == 0 ? 1 : 0); }
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(void* base, uint64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(base, 0, static_cast<int>(min(bytes, static_cast<uint64_t>(0x7fffffff))), 0x00027000);
+}
+
+// Hands in a part: the workgroup's stores have left for memory-side storage before the ticket is drawn.  True for the
+// workgroup that draws the last one; the ticket is then zero again.
+__device__ __forceinline__ bool last_part(uint32_t* ticket, int parts, int* lds_flag) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t t = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *lds_flag = t + 1 == static_cast<uint32_t>(parts);
+    if (t + 1 == static_cast<uint32_t>(parts)) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return *lds_flag != 0;
+}
+
+template <int D>
+struct ThinLds {
+  float o[4][4][D / 64][64][4];  // wavefront, r, piece, lane
+  float ml[4][16][2];
+};
+
+// A run of keys [ka, kb) (from the range's first key rounded down to 32) of one (sequence, kv head) with R <= 16 rows.
+// `self`: this workgroup's place in the cut; x0: the item's first position in the stream.
+template <int kCode, int D, typename T, int kParts, bool kCap>
+__device__ __forceinline__ void thin_item(const QuantArgs& a, const Seq& q, int s, int h, int ka, int kb, const Cut& cut, int self, int64_t x0,
+                                          char* lds_raw, int* lds_flag) {
+  constexpr int NP = D / 64;   // 16-byte pieces of a K row per lane
+  constexpr int NV = D / 64;   // words of a V row per lane
+  constexpr int NO = D / 16;   // output tiles
+  ThinLds<D>& lds = *reinterpret_cast<ThinLds<D>*>(lds_raw);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int G = a.group, R = q.q_len * G, dim = a.p.head_dim;
+  const Range range = key_range(a, q, 0, q.q_len);
+  const int base = range.first & ~31, keys = range.end - base;
+  const int token = i / G, head = h * G + i - token * G;
+  const bool real = i < R;
+  // keys of row i
+  const int pos = q.kv_len - q.q_len + token;
+  const int hi = real ? pos + 1 : 0;
+  const int lo = a.p.sliding_window > 0 ? max(static_cast<int>(max(static_cast<int64_t>(pos) - a.p.sliding_window + 1, static_cast<int64_t>(0))), 0) : 0;
+  const int full_lo = a.p.sliding_window > 0 ? max(q.kv_len - a.p.sliding_window, 0) : 0;  // keys every row sees
+  const int full_hi = q.kv_len - q.q_len + 1;
+
+  bf16x8_t qf[2 * NP][kParts];
+  {
+    const T* row = static_cast<const T*>(a.p.queries) + (q.q0 + (real ? token : 0)) * a.p.query_token_stride + (real ? head : 0) * a.p.query_head_stride;
+#pragma unroll
+    for (int k = 0; k < 2 * NP; ++k) load_q<T, kParts>(row, real, 16 * (g + 4 * (k >> 1)) + 8 * (k & 1), dim, qf[k]);
+  }
+  f32x4_t acc[NO];
+#pragma unroll
+  for (int n = 0; n < NO; ++n) acc[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m = kNoKey, l = 0.f;
+
+  const int32_t* __restrict__ table = a.p.block_tables + static_cast<size_t>(s) * a.p.pages_per_seq;
+  const int last_page = max(q.kv_len - 1, 0) >> a.page_shift;
+  // pieces beyond head_dim read the row's first again (the queries are zero there, the outputs not stored)
+  int k_off[NP], v_off;
+#pragma unroll
+  for (int n = 0; n < NP; ++n) k_off[n] = 16 * (g + 4 * n) < dim ? 16 * (g + 4 * n) : 0;
+  v_off = NO * i < dim ? NO * i : 0;
+
+  struct Pages {
+    int k[2], v[2];
+  };
+  auto load_pages = [&](int k0) {
+    Pages pg;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      pg.k[u] = page_of_key(a, table, k0 + 16 * u + i, last_page);
+      pg.v[u] = page_of_key(a, table, k0 + 16 * u + 4 * g, last_page);
+    }
+    return pg;
+  };
+  u32x4_t kr[2][NP];
+  uint32_t vr[2][4][NV];
+  float ks[2], vs[2];
+  auto load_k = [&](int k0, const Pages& pg) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const char* row = row_of(a, pg.k[u], 2 * h, k0 + 16 * u + i);
+#pragma unroll
+      for (int n = 0; n < NP; ++n) kr[u][n] = *reinterpret_cast<const u32x4_t*>(row + k_off[n]);
+      ks[u] = *scale_of(a, pg.v[u], 2 * h, k0 + 16 * u + 4 * g);
+    }
+  };
+  auto load_v = [&](int k0, const Pages& pg) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const char* row = row_of(a, pg.v[u], 2 * h + 1, k0 + 16 * u + 4 * g) + v_off;
+      vs[u] = *scale_of(a, pg.v[u], 2 * h + 1, k0 + 16 * u + 4 * g);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(row + r * dim);
+        if constexpr (NV == 1) {
+          vr[u][r][0] = src[0];
+        } else if constexpr (NV == 2) {
+          const u32x2_t w = *reinterpret_cast<const u32x2_t*>(src);
+          vr[u][r][0] = w[0], vr[u][r][1] = w[1];
+        } else {
+          const u32x4_t w = *reinterpret_cast<const u32x4_t*>(src);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) vr[u][r][j] = w[j];
+        }
+      }
+    }
+  };
+
+  const float cap = a.p.logits_soft_cap, inv_cap = kCap ? 1.f / cap : 0.f;
+  const float c_scale = kCap ? a.p.softmax_scale : a.p.softmax_scale * kLog2e, cap2 = cap * kLog2e;
+  const int t_end = (min(kb, keys) + 31) >> 5;
+  int t = (ka >> 5) + wave;
+  Pages pg = {}, pg_next = {};
+  if (t < t_end) {
+    pg = load_pages(base + 32 * t);
+    load_k(base + 32 * t, pg);
+    load_v(base + 32 * t, pg);
+    if (t + 4 < t_end) pg_next = load_pages(base + 32 * (t + 4));
+  }
+  for (; t < t_end; t += 4) {
+    const int k0 = base + 32 * t;
+    f32x4_t sa[2] = {f32x4_t{0.f, 0.f, 0.f, 0.f}, f32x4_t{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+        bf16x8_t op[2];
+        widen16<kCode>(kr[u][n], op);
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+          for (int sp = 0; sp < kParts; ++sp) sa[u] = mfma(op[hf], qf[2 * n + hf][sp], sa[u]);
+      }
+    const float c[2] = {ks[0] * c_scale, ks[1] * c_scale};
+    float w[2] = {vs[0], vs[1]};
+    const bool more = t + 4 < t_end;
+    Pages pg_after = {};
+    if (more) {
+      if (t + 8 < t_end) pg_after = load_pages(k0 + 256);
+      load_k(k0 + 128, pg_next);
+    }
+    float x[2][4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[u][r] = scaled<kCap>(sa[u][r], c[u], cap2, inv_cap);
+    const bool edge = k0 < full_lo || k0 + 32 > full_hi;
+    if (edge) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int k = k0 + 16 * u + 4 * g;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[u][r] = k + r >= lo && k + r < hi ? x[u][r] : -INFINITY;
+          // what no row of the sequence sees may be anything
+          if (k + r < range.first || k + r >= range.end) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) vr[u][r][j] = 0u;
+          }
+        }
+        if (k + 3 < range.first || k >= range.end) w[u] = 0.f;
+      }
+    }
+    const float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+    if (__any(top > m + kLazy)) {
+      const float m_new = fmaxf(m, row_groups_max(top));
+      const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+#pragma unroll
+      for (int n = 0; n < NO; ++n) acc[n] *= alpha;
+      l *= alpha;
+      m = m_new;
+    }
+    float pv[8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float p = __builtin_amdgcn_exp2f(x[u][r] - m);
+        l += p;
+        pv[4 * u + r] = p * w[u];
+      }
+    bf16x8_t pf[kParts];
+    split<kParts>(pv, pf);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      uint32_t pair[4][4];  // keys (0 1) (2 3) (16 17) (18 19) of the group, bytes 0..3
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        widen_pairs<kCode>(vr[u][0][j], vr[u][1][j], pair[2 * u]);
+        widen_pairs<kCode>(vr[u][2][j], vr[u][3][j], pair[2 * u + 1]);
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const bf16x8_t v = __builtin_bit_cast(bf16x8_t, u32x4_t{pair[0][b], pair[1][b], pair[2][b], pair[3][b]});
+#pragma unroll
+        for (int sp = 0; sp < kParts; ++sp) acc[4 * j + b] = mfma(v, pf[sp], acc[4 * j + b]);
+      }
+    }
+    if (more) load_v(k0 + 128, pg_next);
+    pg_next = pg_after;
+  }
+  l = row_groups_sum(l);
+
+  // The four wavefronts meet: wavefront w adds up outputs NO (4 g + w) .. + NO of every row.
+  __syncthreads();  // LDS may hold what came before
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int n = 0; n < NO / 4; ++n)
+      *reinterpret_cast<f32x4_t*>(lds.o[wave][r][n][lane]) = f32x4_t{acc[4 * n][r], acc[4 * n + 1][r], acc[4 * n + 2][r], acc[4 * n + 3][r]};
+  if (g == 0) lds.ml[wave][i][0] = m, lds.ml[wave][i][1] = l;
+  __syncthreads();
+  float top = kNoKey, sum = 0.f, o[NO];
+#pragma unroll
+  for (int v = 0; v < 4; ++v) top = fmaxf(top, lds.ml[v][i][0]);
+#pragma unroll
+  for (int n = 0; n < NO; ++n) o[n] = 0.f;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    const float f = __builtin_amdgcn_exp2f(lds.ml[v][i][0] - top);
+    sum = fmaf(f, lds.ml[v][i][1], sum);
+#pragma unroll
+    for (int n = 0; n < NO / 4; ++n) {
+      const f32x4_t y = *reinterpret_cast<const f32x4_t*>(lds.o[v][wave][n][lane]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[4 * n + e] = fmaf(f, y[e], o[4 * n + e]);
+    }
+  }
+
+  if (ka > 0 || kb < keys) {  // a part: hand it in, and add all of them up if it is the last
+    const Parts parts = parts_of(cut, x0, range.end - range.first, kThinStep);
+    const int slots = 2 * a.grid;
+    const auto o_rsrc = rsrc_of(a.thin_o, static_cast<uint64_t>(slots) * 16 * D * 4);
+    const int part = self - parts.first;
+    const auto place = [&](int k, int n) { return ((slot_of(parts, k) * 4 + wave) * (NO / 4) + n) * 1024 + lane * 16; };
+#pragma unroll
+    for (int n = 0; n < NO / 4; ++n)
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, f32x4_t{o[4 * n], o[4 * n + 1], o[4 * n + 2], o[4 * n + 3]}), o_rsrc, place(part, n), 0, kAgentScope);
+    if (wave == 0 && g == 0) {
+      const uint64_t both = (static_cast<uint64_t>(__float_as_uint(sum)) << 32) | __float_as_uint(top);
+      __hip_atomic_store(reinterpret_cast<uint64_t*>(a.thin_ml) + slot_of(parts, part) * 16 + i, both, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (!last_part(a.tickets + parts.first, parts.count, lds_flag)) return;
+    top = kNoKey, sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < NO; ++n) o[n] = 0.f;
+    for (int k = 0; k < parts.count; ++k) {
+      const uint64_t both = __hip_atomic_load(reinterpret_cast<uint64_t*>(a.thin_ml) + slot_of(parts, k) * 16 + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const float mk = __uint_as_float(static_cast<uint32_t>(both)), lk = __uint_as_float(static_cast<uint32_t>(both >> 32));
+      const float t_new = fmaxf(top, mk), f = __builtin_amdgcn_exp2f(top - t_new), fk = __builtin_amdgcn_exp2f(mk - t_new);
+      top = t_new;
+      sum = sum * f + lk * fk;
+#pragma unroll
+      for (int n = 0; n < NO / 4; ++n) {
+        const f32x4_t y = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(o_rsrc, place(k, n), 0, kAgentScope));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[4 * n + e] = o[4 * n + e] * f + y[e] * fk;
+      }
+    }
+  }
+  if (!real) return;
+  float weight;
+  add_sinks(a, head, top, sum, weight);
+  const float f = sum > 0.f ? weight / sum : 0.f;
+  T* dst = static_cast<T*>(a.p.out) + (static_cast<size_t>(q.q0 + token) * a.p.num_q_heads + head) * dim;
+#pragma unroll
+  for (int n = 0; n < NO; ++n) o[n] *= f;
+  if (NO * (4 * g + wave) < dim) store_row<T, NO>(dst + NO * (4 * g + wave), o);
+}
+
+template <int D>
+struct TileLds {
+  bf16x8_t k[2][quant_step_keys<D>() / 16][D / 32][64];  // buffer, 16 keys, 32 elements, lane
+  bf16x8_t v[2][quant_step_keys<D>() / 32][D / 16][64];  // buffer, 32 keys, output tile, lane
+  float ks[2][quant_step_keys<D>() / 4];
+  float vs[2][quant_step_keys<D>() / 4];
+};
+
+// A run of keys [ka, kb) of one tile of rows.
+template <int kCode, int D, typename T, int kParts, bool kCap>
+__device__ __forceinline__ void tile_item(const QuantArgs& a, const Seq& q, int s, int hs, int tile, int ka, int kb, const Cut& cut, int self, int64_t x0,
+                                          char* lds_raw, int* lds_flag) {
+  constexpr int kStep = quant_step_keys<D>(), kRowTiles = quant_row_tiles<D, kParts>();
+  constexpr int NP = D / 64, NO = D / 16, kSub = kStep / 16, kBlocks = kStep / 32;
+  constexpr int kUnitsK = kSub * NP / 4, kUnitsV = (kBlocks * NP + 3) / 4;  // per wavefront
+  TileLds<D>& lds = *reinterpret_cast<TileLds<D>*>(lds_raw);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int dim = a.p.head_dim;
+  const int h = hs / a.subs, sub = hs - h * a.subs;
+  const int t0 = tile * a.tile_tokens, t1 = min(t0 + a.tile_tokens, q.q_len);
+  const Range range = key_range(a, q, t0, t1);
+  const int base = range.first & ~31, keys = range.end - base;
+  const int q_base = q.kv_len - q.q_len;
+
+  // row tile m of this wavefront, row i
+  int token[kRowTiles], head[kRowTiles], lo[kRowTiles], hi[kRowTiles];
+  bf16x8_t qf[kRowTiles][D / 32][kParts];
+#pragma unroll
+  for (int mt = 0; mt < kRowTiles; ++mt) {
+    const int rr = (wave * kRowTiles + mt) * 16 + i;
+    const int dt = rr / a.tile_group, gg = sub * a.tile_group + rr - dt * a.tile_group;
+    const bool real = dt < t1 - t0 && gg < a.group;
+    token[mt] = real ? t0 + dt : -1;
+    head[mt] = h * a.group + gg;
+    const int pos = q_base + t0 + dt;
+    hi[mt] = real ? pos + 1 : 0;
+    lo[mt] = a.p.sliding_window > 0 ? static_cast<int>(max(static_cast<int64_t>(pos) - a.p.sliding_window + 1, static_cast<int64_t>(0))) : 0;
+    const T* row = static_cast<const T*>(a.p.queries) + (q.q0 + (real ? token[mt] : 0)) * a.p.query_token_stride + (real ? head[mt] : 0) * a.p.query_head_stride;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) load_q<T, kParts>(row, real, 16 * (g + 4 * (k >> 1)) + 8 * (k & 1), dim, qf[mt][k]);
+  }
+  const int full_lo = a.p.sliding_window > 0 ? max(q_base + t1 - a.p.sliding_window, 0) : 0;  // keys every row sees
+  const int full_hi = q_base + t0 + 1;
+  f32x4_t acc[kRowTiles][NO];
+  float m[kRowTiles], l[kRowTiles];
+#pragma unroll
+  for (int mt = 0; mt < kRowTiles; ++mt) {
+    m[mt] = kNoKey, l[mt] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NO; ++n) acc[mt][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const int32_t* __restrict__ table = a.p.block_tables + static_cast<size_t>(s) * a.p.pages_per_seq;
+  const int last_page = max(q.kv_len - 1, 0) >> a.page_shift;
+  u32x4_t kr[kUnitsK];
+  uint32_t vr[kUnitsV][2][4];
+  float sc = 0.f;
+  int scale_key = 0;
+  // K unit x: 16 keys, 16 elements a lane; V unit x: 32 keys (8 a lane), 64 elements (4 a lane)
+  auto load_codes = [&](int k0) {
+#pragma unroll
+    for (int n = 0; n < kUnitsK; ++n) {
+      const int x = wave * kUnitsK + n, u = x / NP, piece = g + 4 * (x % NP);
+      const int k = k0 + 16 * u + i;
+      kr[n] = *reinterpret_cast<const u32x4_t*>(row_of(a, page_of_key(a, table, k, last_page), 2 * h, k) + (16 * piece < dim ? 16 * piece : 0));
+    }
+#pragma unroll
+    for (int n = 0; n < kUnitsV; ++n) {
+      const int x = (wave * kUnitsV + n) % (kBlocks * NP), b = x / NP, d = 64 * (x % NP) + 4 * i;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int k = k0 + 32 * b + 16 * u + 4 * g;
+        const char* row = row_of(a, page_of_key(a, table, k, last_page), 2 * h + 1, k) + (d < dim ? d : 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) vr[n][u][r] = *reinterpret_cast<const uint32_t*>(row + r * dim);
+      }
+    }
+    if (threadIdx.x < kStep / 2) {  // groups of 4 keys: the scales of K, then of V
+      const int half = threadIdx.x / (kStep / 4), k = k0 + 4 * (threadIdx.x - half * (kStep / 4));
+      sc = *scale_of(a, page_of_key(a, table, k, last_page), 2 * h + half, k);
+      scale_key = k;
+    }
+  };
+  const float cap = a.p.logits_soft_cap, inv_cap = kCap ? 1.f / cap : 0.f;
+  const float c_scale = kCap ? a.p.softmax_scale : a.p.softmax_scale * kLog2e, cap2 = cap * kLog2e;
+  auto store_codes = [&](int k0, int buf) {
+    const bool edge = k0 < range.first || k0 + kStep > range.end;
+#pragma unroll
+    for (int n = 0; n < kUnitsK; ++n) {
+      const int x = wave * kUnitsK + n, u = x / NP, np = x % NP;
+      bf16x8_t op[2];
+      widen16<kCode>(kr[n], op);
+      lds.k[buf][u][2 * np][lane] = op[0];
+      lds.k[buf][u][2 * np + 1][lane] = op[1];
+    }
+#pragma unroll
+    for (int n = 0; n < kUnitsV; ++n) {
+      const int x = wave * kUnitsV + n, b = x / NP, j = x % NP;
+      if (x >= kBlocks * NP) break;
+      if (edge) {  // what no row of the tile sees may be anything
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int k = k0 + 32 * b + 16 * u + 4 * g + r;
+            if (k < range.first || k >= range.end) vr[n][u][r] = 0u;
+          }
+      }
+      uint32_t pair[4][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        widen_pairs<kCode>(vr[n][u][0], vr[n][u][1], pair[2 * u]);
+        widen_pairs<kCode>(vr[n][u][2], vr[n][u][3], pair[2 * u + 1]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        lds.v[buf][b][4 * j + e][lane] = __builtin_bit_cast(bf16x8_t, u32x4_t{pair[0][e], pair[1][e], pair[2][e], pair[3][e]});
+    }
+    if (threadIdx.x < kStep / 2) {
+      float y = sc;
+      if (scale_key + 3 < range.first || scale_key >= range.end) y = 0.f;
+      float* dst = threadIdx.x < kStep / 4 ? lds.ks[buf] + threadIdx.x : lds.vs[buf] + threadIdx.x - kStep / 4;
+      *dst = threadIdx.x < kStep / 4 ? y * c_scale : y;
+    }
+  };
+
+  const int t_begin = ka / kStep, t_end = (min(kb, keys) + kStep - 1) / kStep;
+  __syncthreads();  // LDS may hold what came before
+  if (t_begin < t_end) {
+    load_codes(base + t_begin * kStep);
+    store_codes(base + t_begin * kStep, 0);
+    if (t_begin + 1 < t_end) load_codes(base + (t_begin + 1) * kStep);
+  }
+  for (int t = t_begin; t < t_end; ++t) {
+    const int k0 = base + t * kStep, buf = (t - t_begin) & 1;
+    __syncthreads();
+    const bool edge = k0 < full_lo || k0 + kStep > full_hi;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+      f32x4_t sa[kRowTiles][2];
+#pragma unroll
+      for (int mt = 0; mt < kRowTiles; ++mt) sa[mt][0] = sa[mt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+          const bf16x8_t op = lds.k[buf][2 * b + u][k][lane];
+#pragma unroll
+          for (int mt = 0; mt < kRowTiles; ++mt)
+#pragma unroll
+            for (int sp = 0; sp < kParts; ++sp) sa[mt][u] = mfma(op, qf[mt][k][sp], sa[mt][u]);
+        }
+      bf16x8_t pf[kRowTiles][kParts];
+      const float c[2] = {lds.ks[buf][8 * b + g], lds.ks[buf][8 * b + 4 + g]}, w[2] = {lds.vs[buf][8 * b + g], lds.vs[buf][8 * b + 4 + g]};
+#pragma unroll
+      for (int mt = 0; mt < kRowTiles; ++mt) {
+        float x[2][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[u][r] = scaled<kCap>(sa[mt][u][r], c[u], cap2, inv_cap);
+        if (edge) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int k = k0 + 32 * b + 16 * u + 4 * g + r;
+              x[u][r] = k >= lo[mt] && k < hi[mt] ? x[u][r] : -INFINITY;
+            }
+        }
+        const float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+        if (__any(top > m[mt] + kLazy)) {
+          const float m_new = fmaxf(m[mt], row_groups_max(top));
+          const float alpha = __builtin_amdgcn_exp2f(m[mt] - m_new);
+#pragma unroll
+          for (int n = 0; n < NO; ++n) acc[mt][n] *= alpha;
+          l[mt] *= alpha;
+          m[mt] = m_new;
+        }
+        float pv[8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float p = __builtin_amdgcn_exp2f(x[u][r] - m[mt]);
+            l[mt] += p;
+            pv[4 * u + r] = p * w[u];
+          }
+        split<kParts>(pv, pf[mt]);
+      }
+      if (b == kBlocks - 1 && t + 1 < t_end) {  // the next step's codes have come in meanwhile
+        store_codes(k0 + kStep, buf ^ 1);
+        if (t + 2 < t_end) load_codes(k0 + 2 * kStep);
+      }
+#pragma unroll
+      for (int n = 0; n < NO; ++n) {
+        const bf16x8_t v = lds.v[buf][b][n][lane];
+#pragma unroll
+        for (int mt = 0; mt < kRowTiles; ++mt)
+#pragma unroll
+          for (int sp = 0; sp < kParts; ++sp) acc[mt][n] = mfma(v, pf[mt][sp], acc[mt][n]);
+      }
+    }
+  }
+#pragma unroll
+  for (int mt = 0; mt < kRowTiles; ++mt) l[mt] = row_groups_sum(l[mt]);
+
+  if (ka > 0 || kb < keys) {
+    const Parts parts = parts_of(cut, x0, range.end - range.first, kStep);
+    const int slots = 2 * a.grid;
+    const auto o_rsrc = rsrc_of(a.tile_o, static_cast<uint64_t>(slots) * 64 * kRowTiles * D * 4);
+    const int part = self - parts.first;
+    const auto place = [&](int k, int mt, int n) { return (((slot_of(parts, k) * 4 + wave) * kRowTiles + mt) * NO + n) * 1024 + lane * 16; };
+    const auto ml_at = [&](int k, int mt) { return reinterpret_cast<uint64_t*>(a.tile_ml) + (slot_of(parts, k) * 4 + wave) * kRowTiles * 16 + mt * 16 + i; };
+#pragma unroll
+    for (int mt = 0; mt < kRowTiles; ++mt) {
+#pragma unroll
+      for (int n = 0; n < NO; ++n) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, acc[mt][n]), o_rsrc, place(part, mt, n), 0, kAgentScope);
+      if (g == 0) {
+        const uint64_t both = (static_cast<uint64_t>(__float_as_uint(l[mt])) << 32) | __float_as_uint(m[mt]);
+        __hip_atomic_store(ml_at(part, mt), both, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    }
+    if (!last_part(a.tickets + a.grid + parts.first, parts.count, lds_flag)) return;
+#pragma unroll
+    for (int mt = 0; mt < kRowTiles; ++mt) {
+      m[mt] = kNoKey, l[mt] = 0.f;
+#pragma unroll
+      for (int n = 0; n < NO; ++n) acc[mt][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < parts.count; ++k) {
+        const uint64_t both = __hip_atomic_load(ml_at(k, mt), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const float mk = __uint_as_float(static_cast<uint32_t>(both)), lk = __uint_as_float(static_cast<uint32_t>(both >> 32));
+        const float t_new = fmaxf(m[mt], mk), f = __builtin_amdgcn_exp2f(m[mt] - t_new), fk = __builtin_amdgcn_exp2f(mk - t_new);
+        m[mt] = t_new;
+        l[mt] = l[mt] * f + lk * fk;
+#pragma unroll
+        for (int n = 0; n < NO; ++n) {
+          const f32x4_t y = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(o_rsrc, place(k, mt, n), 0, kAgentScope));
+          acc[mt][n] = acc[mt][n] * f + y * fk;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int mt = 0; mt < kRowTiles; ++mt) {
+    if (token[mt] < 0) continue;
+    float weight;
+    add_sinks(a, head[mt], m[mt], l[mt], weight);
+    const float f = l[mt] > 0.f ? weight / l[mt] : 0.f;
+    T* dst = static_cast<T*>(a.p.out) + (static_cast<size_t>(q.q0 + token[mt]) * a.p.num_q_heads + head[mt]) * dim;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      float o[16];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[4 * r + e] = acc[mt][4 * j + e][r] * f;
+      if (64 * j + 16 * g < dim) store_row<T, 16>(dst + 64 * j + 16 * g, o);
+    }
+  }
+}
+
+// Place of workgroup b in a stream's cut over n workgroups (-1: none): the workgroups of one XCD hold neighbouring runs.
+__device__ __forceinline__ int place_in_cut(int b, int n) {
+  const int xcd = b & 7, j = b >> 3, per = n >> 3, rem = n & 7;
+  return j < per + (xcd < rem ? 1 : 0) ? xcd * per + min(xcd, rem) + j : -1;
+}
+
+struct SchedLds {
+  int64_t sums[4][2];
+  int longest[4];
+  int items[4];
+  int seq[2];
+  int64_t off[2];
+  int flag;
+};
+
+template <int kCode, int D, typename T, int kParts, bool kCap>
+__global__ __launch_bounds__(256, 2) void quant_attention_kernel(QuantArgs a) {
+  constexpr size_t kLds = sizeof(TileLds<D>) > sizeof(ThinLds<D>) ? sizeof(TileLds<D>) : sizeof(ThinLds<D>);
+  __shared__ __align__(16) char lds[kLds];
+  __shared__ SchedLds sched;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = min(max(a.p.num_seqs[0], 0), a.p.max_num_seqs);
+  const int heads[2] = {a.p.num_kv_heads, a.p.num_kv_heads * a.subs};
+
+  // Lengths of the two streams, and the longest item and the number of items of the first.
+  const int per = (n + 255) >> 8;
+  const int s0 = min(static_cast<int>(threadIdx.x) * per, n), s1 = min(s0 + per, n);
+  int64_t sum[2] = {0, 0};
+  int longest = 0, items = 0;
+  for (int s = s0; s < s1; ++s) {
+    const Seq q = load_seq(a, n, s);
+    if (q.q_len == 0) continue;
+    if (is_thin(a, q)) {
+      const int k = thin_keys(a, q);
+      sum[0] += static_cast<int64_t>(k + kThinPad) * heads[0];
+      longest = max(longest, k);
+      items += heads[0];
+    } else {
+      sum[1] += tiles_before(a, q, tiles_of(a, q), true) * heads[1];
+    }
+  }
+  int64_t inc[2] = {sum[0], sum[1]};
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t x = __shfl_up(inc[0], o), y = __shfl_up(inc[1], o);
+    if (lane >= o) inc[0] += x, inc[1] += y;
+    longest = max(longest, __shfl_xor(longest, o));
+    items += __shfl_xor(items, o);
+  }
+  if (lane == 63) {
+    sched.sums[wave][0] = inc[0], sched.sums[wave][1] = inc[1];
+    sched.longest[wave] = longest, sched.items[wave] = items;
+  }
+  __syncthreads();
+  int64_t before[2] = {inc[0] - sum[0], inc[1] - sum[1]}, total[2] = {0, 0};
+  longest = items = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) before[0] += sched.sums[w][0], before[1] += sched.sums[w][1];
+    total[0] += sched.sums[w][0], total[1] += sched.sums[w][1];
+    longest = max(longest, sched.longest[w]);
+    items += sched.items[w];
+  }
+  Cut cut[2];
+  cut[0].total = total[0];
+  cut[0].n = static_cast<int>(min(static_cast<int64_t>(a.grid), max(total[0] / kThinLeast, static_cast<int64_t>(1))));
+  cut[1].total = total[1];
+  cut[1].n = static_cast<int>(min(static_cast<int64_t>(a.grid), max(total[1] / kTileLeast, static_cast<int64_t>(1))));
+  // the first stream from the grid's front, the second from its back: where both are short they meet different workgroups
+  const int mine[2] = {total[0] > 0 ? place_in_cut(blockIdx.x, cut[0].n) : -1, total[1] > 0 ? place_in_cut(a.grid - 1 - blockIdx.x, cut[1].n) : -1};
+  int64_t x_begin[2] = {0, 0}, x_end[2] = {0, 0};
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    if (mine[c] >= 0) x_begin[c] = cut[c].bound(mine[c]), x_end[c] = cut[c].bound(mine[c] + 1);
+  // the thread whose sequences hold a run's first position finds it
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    if (mine[c] < 0 || x_begin[c] < before[c] || x_begin[c] >= before[c] + sum[c]) continue;
+    int64_t off = x_begin[c] - before[c];
+    for (int s = s0; s < s1; ++s) {
+      const Seq q = load_seq(a, n, s);
+      if (q.q_len == 0 || is_thin(a, q) != (c == 0)) continue;
+      const int64_t len = c == 0 ? static_cast<int64_t>(thin_keys(a, q) + kThinPad) * heads[0] : tiles_before(a, q, tiles_of(a, q), true) * heads[1];
+      if (off < len) {
+        sched.seq[c] = s;
+        sched.off[c] = off;
+        break;
+      }
+      off -= len;
+    }
+  }
+  __syncthreads();
+
+  Window window;
+  auto thin_phase = [&] {
+    if (x_begin[0] >= x_end[0]) return;
+    int s = __builtin_amdgcn_readfirstlane(sched.seq[0]);
+    int64_t off = sched.off[0], x = x_begin[0];
+    while (x < x_end[0] && s < n) {
+      window.at(a, n, s);
+      const Seq q = window.get(s);
+      const int keys = thin_keys(a, q), len = keys + kThinPad;
+      const Range range = key_range(a, q, 0, q.q_len);
+      const int all = range.end - (range.first & ~31);  // keys as they are walked
+      int h = static_cast<int>(off / len);
+      int begin = static_cast<int>(off - static_cast<int64_t>(h) * len);
+      for (; h < heads[0] && x < x_end[0]; ++h, begin = 0) {
+        const int end = static_cast<int>(min(static_cast<int64_t>(len), begin + (x_end[0] - x)));
+        const int ka = begin >= keys ? all : begin / kThinStep * kThinStep, kb = end >= keys ? all : end / kThinStep * kThinStep;
+        if (ka < kb || (keys == 0 && begin == 0))
+          thin_item<kCode, D, T, kParts, kCap>(a, q, s, h, keys == 0 ? 0 : ka, kb, cut[0], mine[0], x - begin, lds, &sched.flag);
+        x += end - begin;
+      }
+      off = 0;
+      s = window.next(a, n, s + 1, true);
+    }
+  };
+  auto tile_phase = [&] {
+    if (x_begin[1] >= x_end[1]) return;
+    constexpr int kStep = quant_step_keys<D>();
+    int s = __builtin_amdgcn_readfirstlane(sched.seq[1]);
+    int64_t off = sched.off[1], x = x_begin[1];
+    while (x < x_end[1] && s < n) {
+      window.at(a, n, s);
+      const Seq q = window.get(s);
+      const int tiles = tiles_of(a, q);
+      const int64_t len = tiles_before(a, q, tiles, true);
+      int h = static_cast<int>(off / len);
+      int64_t rest = off - static_cast<int64_t>(h) * len;
+      int tile = 0;
+      for (int hi = tiles; hi - tile > 1;) {  // the last tile that starts at or before the position
+        const int mid = (tile + hi) >> 1;
+        if (tiles_before(a, q, mid, false) <= rest) tile = mid;
+        else hi = mid;
+      }
+      int begin = static_cast<int>(rest - tiles_before(a, q, tile, false));
+      for (; h < heads[1] && x < x_end[1]; ++h, tile = 0) {
+        for (; tile < tiles && x < x_end[1]; ++tile, begin = 0) {
+          const Range range = key_range(a, q, tile * a.tile_tokens, min((tile + 1) * a.tile_tokens, q.q_len));
+          const int keys = range.end - range.first, all = range.end - (range.first & ~31), item = keys + kTilePad;
+          const int end = static_cast<int>(min(static_cast<int64_t>(item), begin + (x_end[1] - x)));
+          const int ka = begin >= keys ? all : begin / kStep * kStep, kb = end >= keys ? all : end / kStep * kStep;
+          if (ka < kb || (keys == 0 && begin == 0))
+            tile_item<kCode, D, T, kParts, kCap>(a, q, s, h, tile, keys == 0 ? 0 : ka, kb, cut[1], mine[1], x - begin, lds, &sched.flag);
+          x += end - begin;
+        }
+      }
+      off = 0;
+      s = window.next(a, n, s + 1, false);
+    }
+  };
+  const bool thin_first = static_cast<int>(blockIdx.x) * 2 < a.grid;
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+    if ((k == 0) == thin_first) thin_phase();
+    else tile_phase();
+  }
+
+  // Rows in front of the first sequence and behind the last are zeros.
+  const int row_first = n > 0 ? min(max(a.p.query_start_loc[0], 0), a.p.total_tokens) : 0;
+  const int row_last = n > 0 ? max(row_first, min(max(a.p.query_start_loc[n], 0), a.p.total_tokens)) : 0;
+  const int64_t row_words = static_cast<int64_t>(a.p.num_q_heads) * a.p.head_dim * sizeof(T) / 16;
+  u32x4_t* out = static_cast<u32x4_t*>(a.p.out);
+  const int64_t at = blockIdx.x * 256 + threadIdx.x, stride = static_cast<int64_t>(a.grid) * 256;
+  for (int64_t k = at; k < row_first * row_words; k += stride) out[k] = u32x4_t{0u, 0u, 0u, 0u};
+  for (int64_t k = row_last * row_words + at; k < a.p.total_tokens * row_words; k += stride) out[k] = u32x4_t{0u, 0u, 0u, 0u};
+}
+
+}  // namespace quant
+
+// Launches the kernel for one type of codes; head_dim is padded to 64, 128 or 256.
+template <int kCode>
+int launch_quant_codes(const QuantArgs& a, hipStream_t stream) {
+  const bool f32 = a.p.dtype == RPA_DTYPE_F32, cap = a.p.logits_soft_cap != 0.f;
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(a.grid), dim3(256), 0, stream, a);
+    return hipGetLastError() == hipSuccess ? RPA_OK : RPA_ERR_LAUNCH;
+  };
+  auto width = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    if (f32) return cap ? go(quant::quant_attention_kernel<kCode, D, float, 3, true>) : go(quant::quant_attention_kernel<kCode, D, float, 3, false>);
+    return cap ? go(quant::quant_attention_kernel<kCode, D, bf16_t, 1, true>) : go(quant::quant_attention_kernel<kCode, D, bf16_t, 1, false>);
+  };
+  if (a.p.head_dim <= 64) return width(std::integral_constant<int, 64>{});
+  if (a.p.head_dim <= 128) return width(std::integral_constant<int, 128>{});
+  return width(std::integral_constant<int, 256>{});
+}
+
+int launch_quant_i8(const QuantArgs& a, hipStream_t stream);
+int launch_quant_e4m3(const QuantArgs& a, hipStream_t stream);
+int launch_quant_e5m2(const QuantArgs& a, hipStream_t stream);
+
+}  // namespace rpa
