@@ -42,9 +42,9 @@ struct QuantArgs {
 
 // Shape of the second stream's tiles for a (padded) head_dim: keys per step, and 16-row tiles per wavefront.
 template <int D>
-constexpr int quant_step_keys() { return 8192 / D; }
+constexpr int quant_step_keys() { return D == 256 ? 32 : 64; }
 template <int D, int kParts>
-constexpr int quant_row_tiles() { return kParts == 3 ? 1 : 2; }
+constexpr int quant_row_tiles() { return kParts == 3 || D == 256 ? 1 : 2; }
 
 constexpr int kThinStep = 128;     // keys a workgroup takes at once in the first stream
 constexpr int kThinPad = 128;      // what an item of the first stream costs beyond its keys, in keys
@@ -56,6 +56,9 @@ constexpr float kLazy = 8.f;       // the running maximum follows when a logit p
 constexpr int kAgentScope = 16;    // auxiliary bit of a buffer access: coherent across the device's L2s
 
 namespace quant {
+
+// The launch's arguments where the hardware keeps them: constant memory, read through the scalar cache.
+typedef const __attribute__((address_space(4))) QuantArgs Args;
 
 struct Seq {
   int q0, q_len, kv_len;
@@ -71,7 +74,7 @@ __device__ __forceinline__ int64_t ramp(int64_t n, int64_t c, int64_t d) {  // s
 struct Range {
   int first, end;
 };
-__device__ __forceinline__ Range key_range(const QuantArgs& a, const Seq& q, int t0, int t1) {
+__device__ __forceinline__ Range key_range(Args& a, const Seq& q, int t0, int t1) {
   const int base = q.kv_len - q.q_len;
   Range r;
   r.end = max(base + t1, 0);
@@ -81,9 +84,9 @@ __device__ __forceinline__ Range key_range(const QuantArgs& a, const Seq& q, int
 }
 
 // The second stream: tiles of one (sequence, head).
-__device__ __forceinline__ int tiles_of(const QuantArgs& a, const Seq& q) { return (q.q_len + a.tile_tokens - 1) / a.tile_tokens; }
+__device__ __forceinline__ int tiles_of(Args& a, const Seq& q) { return (q.q_len + a.tile_tokens - 1) / a.tile_tokens; }
 // Stream positions in front of tile n (n below the number of tiles), or of all tiles.
-__device__ __forceinline__ int64_t tiles_before(const QuantArgs& a, const Seq& q, int n, bool all) {
+__device__ __forceinline__ int64_t tiles_before(Args& a, const Seq& q, int n, bool all) {
   const int64_t base = q.kv_len - q.q_len, d = a.tile_tokens;
   int64_t sum = ramp(n, base + d, d) + static_cast<int64_t>(n) * kTilePad;
   if (a.p.sliding_window > 0) sum -= ramp(n, base - a.p.sliding_window + 1, d);
@@ -91,14 +94,14 @@ __device__ __forceinline__ int64_t tiles_before(const QuantArgs& a, const Seq& q
   return sum;
 }
 
-__device__ __forceinline__ bool is_thin(const QuantArgs& a, const Seq& q) { return static_cast<int64_t>(q.q_len) * a.group <= 16; }
+__device__ __forceinline__ bool is_thin(Args& a, const Seq& q) { return static_cast<int64_t>(q.q_len) * a.group <= 16; }
 
-__device__ __forceinline__ int thin_keys(const QuantArgs& a, const Seq& q) {
+__device__ __forceinline__ int thin_keys(Args& a, const Seq& q) {
   const Range r = key_range(a, q, 0, q.q_len);
   return r.end - r.first;
 }
 
-__device__ __forceinline__ Seq load_seq(const QuantArgs& a, int n, int s) {
+__device__ __forceinline__ Seq load_seq(Args& a, int n, int s) {
   Seq q = {0, 0, 0};
   if (s < n) {
     q.q0 = min(max(a.p.query_start_loc[s], 0), a.p.total_tokens);
@@ -121,7 +124,7 @@ struct Cut {
 struct Window {
   Seq mine;
   int base = -1;
-  __device__ __forceinline__ void at(const QuantArgs& a, int n, int s) {
+  __device__ __forceinline__ void at(Args& a, int n, int s) {
     if (base >= 0 && s >= base && s < base + 64) return;
     base = s;
     mine = load_seq(a, n, s + (threadIdx.x & 63));
@@ -131,7 +134,7 @@ struct Window {
     return {__builtin_amdgcn_readlane(mine.q0, l), __builtin_amdgcn_readlane(mine.q_len, l), __builtin_amdgcn_readlane(mine.kv_len, l)};
   }
   // The first sequence from s on that is in the stream, or n.
-  __device__ __forceinline__ int next(const QuantArgs& a, int n, int s, bool thin) {
+  __device__ __forceinline__ int next(Args& a, int n, int s, bool thin) {
     while (s < n) {
       at(a, n, s);
       const uint64_t m = __ballot(mine.q_len > 0 && is_thin(a, mine) == thin) >> (s - base);
@@ -143,15 +146,15 @@ struct Window {
 };
 
 // First key row of (page of key k, combined head) in the pool, in rows of the head's page.
-__device__ __forceinline__ int page_of_key(const QuantArgs& a, const int32_t* __restrict__ table, int k, int last_page) {
+__device__ __forceinline__ int page_of_key(Args& a, const int32_t* __restrict__ table, int k, int last_page) {
   return clamp_page(table[min(k >> a.page_shift, last_page)], a.p.num_pages);
 }
-__device__ __forceinline__ const char* row_of(const QuantArgs& a, int page, int head, int k) {
+__device__ __forceinline__ const char* row_of(Args& a, int page, int head, int k) {
   const uint64_t line = static_cast<uint64_t>(page) * (2 * a.p.num_kv_heads) + head;
   const uint64_t row = (line << a.page_shift) + (k & ((1 << a.page_shift) - 1));
   return static_cast<const char*>(a.p.kv_cache) + row * a.p.head_dim;
 }
-__device__ __forceinline__ const float* scale_of(const QuantArgs& a, int page, int head, int k) {
+__device__ __forceinline__ const float* scale_of(Args& a, int page, int head, int k) {
   const uint64_t line = static_cast<uint64_t>(page) * (2 * a.p.num_kv_heads) + head;
   return a.p.kv_scales + (line << (a.page_shift - a.block_shift)) + ((k & ((1 << a.page_shift) - 1)) >> a.block_shift);
 }
@@ -236,7 +239,7 @@ __device__ __forceinline__ float scaled(float s, float c, float cap, float inv_c
 }
 
 // Adds the row's sinks to its sum: (m, l) -> weight of the output and sum under the larger of the two maxima.
-__device__ __forceinline__ void add_sinks(const QuantArgs& a, int head, float m, float& l, float& weight) {
+__device__ __forceinline__ void add_sinks(Args& a, int head, float m, float& l, float& weight) {
   weight = 1.f;
   if (a.p.num_sinks == 0 || !(l > 0.f)) return;
   const float* sink = a.p.sinks + static_cast<size_t>(head) * a.p.num_sinks;
@@ -300,52 +303,38 @@ __device__ __forceinline__ bool last_part(uint32_t* ticket, int parts, int* lds_
   return *lds_flag != 0;
 }
 
-template <int D>
-struct ThinLds {
-  float o[4][4][D / 64][64][4];  // wavefront, r, piece, lane
-  float ml[4][16][2];
+// One wavefront's pass over keys k_begin, k_begin + stride, ... < k_end, 32 at a time (all multiples of 32): MT tiles of 16
+// rows against one kv head of sequence s.  Lane (i, g) = (lane % 16, lane / 16) holds column i, a query row, of every
+// product.  K: rows i of two 16-key subtiles, pieces g, g + 4, ... of 16 elements, straight from the cache in the order in
+// which the matrix unit takes them (q is loaded in the same order).  The logits come out as keys 4 g + r and 16 + 4 g + r,
+// which is how the second product wants them, so probabilities stay in their lanes; V: those eight keys, D / 16
+// neighbouring elements of each, which byte permutes turn into operands along the keys.  K of the next tile is asked for
+// when this tile's has been multiplied, V likewise: one set of registers each, filled for half of the time.
+template <int MT, int kD>
+struct RowState {
+  f32x4_t acc[MT][kD / 16];  // output element (kD / 16) (4 g + r) + n of row i, unnormalised
+  float m[MT], l[MT];        // running maximum (log2) of the row, this lane's share of its sum
 };
-
-// A run of keys [ka, kb) (from the range's first key rounded down to 32) of one (sequence, kv head) with R <= 16 rows.
-// `self`: this workgroup's place in the cut; x0: the item's first position in the stream.
-template <int kCode, int D, typename T, int kParts, bool kCap>
-__device__ __forceinline__ void thin_item(const QuantArgs& a, const Seq& q, int s, int h, int ka, int kb, const Cut& cut, int self, int64_t x0,
-                                          char* lds_raw, int* lds_flag) {
-  constexpr int NP = D / 64;   // 16-byte pieces of a K row per lane
-  constexpr int NV = D / 64;   // words of a V row per lane
-  constexpr int NO = D / 16;   // output tiles
-  ThinLds<D>& lds = *reinterpret_cast<ThinLds<D>*>(lds_raw);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-  const int G = a.group, R = q.q_len * G, dim = a.p.head_dim;
-  const Range range = key_range(a, q, 0, q.q_len);
-  const int base = range.first & ~31, keys = range.end - base;
-  const int token = i / G, head = h * G + i - token * G;
-  const bool real = i < R;
-  // keys of row i
-  const int pos = q.kv_len - q.q_len + token;
-  const int hi = real ? pos + 1 : 0;
-  const int lo = a.p.sliding_window > 0 ? max(static_cast<int>(max(static_cast<int64_t>(pos) - a.p.sliding_window + 1, static_cast<int64_t>(0))), 0) : 0;
-  const int full_lo = a.p.sliding_window > 0 ? max(q.kv_len - a.p.sliding_window, 0) : 0;  // keys every row sees
-  const int full_hi = q.kv_len - q.q_len + 1;
-
-  bf16x8_t qf[2 * NP][kParts];
-  {
-    const T* row = static_cast<const T*>(a.p.queries) + (q.q0 + (real ? token : 0)) * a.p.query_token_stride + (real ? head : 0) * a.p.query_head_stride;
+template <int kCode, int D, int kParts, bool kCap, int MT>
+__device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const bf16x8_t (&qf)[MT][D / 32][kParts], const int (&lo)[MT],
+                                     const int (&hi)[MT], const Range& range, int full_lo, int full_hi, int k_begin, int k_end, int stride,
+                                     RowState<MT, D>& st) {
+  constexpr int NP = D / 64, NV = D / 64, NO = D / 16;
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, dim = a.p.head_dim;
 #pragma unroll
-    for (int k = 0; k < 2 * NP; ++k) load_q<T, kParts>(row, real, 16 * (g + 4 * (k >> 1)) + 8 * (k & 1), dim, qf[k]);
+  for (int mt = 0; mt < MT; ++mt) {
+    st.m[mt] = kNoKey, st.l[mt] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NO; ++n) st.acc[mt][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  f32x4_t acc[NO];
-#pragma unroll
-  for (int n = 0; n < NO; ++n) acc[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m = kNoKey, l = 0.f;
-
+  if (k_begin >= k_end) return;
   const int32_t* __restrict__ table = a.p.block_tables + static_cast<size_t>(s) * a.p.pages_per_seq;
   const int last_page = max(q.kv_len - 1, 0) >> a.page_shift;
   // pieces beyond head_dim read the row's first again (the queries are zero there, the outputs not stored)
-  int k_off[NP], v_off;
+  int k_off[NP];
 #pragma unroll
   for (int n = 0; n < NP; ++n) k_off[n] = 16 * (g + 4 * n) < dim ? 16 * (g + 4 * n) : 0;
-  v_off = NO * i < dim ? NO * i : 0;
+  const int v_off = NO * i < dim ? NO * i : 0;
 
   struct Pages {
     int k[2], v[2];
@@ -395,18 +384,17 @@ __device__ __forceinline__ void thin_item(const QuantArgs& a, const Seq& q, int 
 
   const float cap = a.p.logits_soft_cap, inv_cap = kCap ? 1.f / cap : 0.f;
   const float c_scale = kCap ? a.p.softmax_scale : a.p.softmax_scale * kLog2e, cap2 = cap * kLog2e;
-  const int t_end = (min(kb, keys) + 31) >> 5;
-  int t = (ka >> 5) + wave;
-  Pages pg = {}, pg_next = {};
-  if (t < t_end) {
-    pg = load_pages(base + 32 * t);
-    load_k(base + 32 * t, pg);
-    load_v(base + 32 * t, pg);
-    if (t + 4 < t_end) pg_next = load_pages(base + 32 * (t + 4));
+  Pages pg_next = {};
+  {
+    const Pages pg = load_pages(k_begin);
+    load_k(k_begin, pg);
+    load_v(k_begin, pg);
+    if (k_begin + stride < k_end) pg_next = load_pages(k_begin + stride);
   }
-  for (; t < t_end; t += 4) {
-    const int k0 = base + 32 * t;
-    f32x4_t sa[2] = {f32x4_t{0.f, 0.f, 0.f, 0.f}, f32x4_t{0.f, 0.f, 0.f, 0.f}};
+  for (int k0 = k_begin; k0 < k_end; k0 += stride) {
+    f32x4_t sa[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) sa[mt][0] = sa[mt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -416,58 +404,76 @@ __device__ __forceinline__ void thin_item(const QuantArgs& a, const Seq& q, int 
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-          for (int sp = 0; sp < kParts; ++sp) sa[u] = mfma(op[hf], qf[2 * n + hf][sp], sa[u]);
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int sp = 0; sp < kParts; ++sp) sa[mt][u] = mfma(op[hf], qf[mt][2 * n + hf][sp], sa[mt][u]);
       }
-    const float c[2] = {ks[0] * c_scale, ks[1] * c_scale};
-    float w[2] = {vs[0], vs[1]};
-    const bool more = t + 4 < t_end;
+    float c[2] = {ks[0] * c_scale, ks[1] * c_scale}, w[2] = {vs[0], vs[1]};
+    const bool more = k0 + stride < k_end;
     Pages pg_after = {};
     if (more) {
-      if (t + 8 < t_end) pg_after = load_pages(k0 + 256);
-      load_k(k0 + 128, pg_next);
+      if (k0 + 2 * stride < k_end) pg_after = load_pages(k0 + 2 * stride);
+      load_k(k0 + stride, pg_next);
     }
-    float x[2][4];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[u][r] = scaled<kCap>(sa[u][r], c[u], cap2, inv_cap);
     const bool edge = k0 < full_lo || k0 + 32 > full_hi;
-    if (edge) {
+    if (kCap || edge) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int k = k0 + 16 * u + 4 * g;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          x[u][r] = k + r >= lo && k + r < hi ? x[u][r] : -INFINITY;
-          // what no row of the sequence sees may be anything
-          if (k + r < range.first || k + r >= range.end) {
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int j = 0; j < NV; ++j) vr[u][r][j] = 0u;
+          for (int r = 0; r < 4; ++r) {
+            const float x = scaled<kCap>(sa[mt][u][r], c[u], cap2, inv_cap);
+            sa[mt][u][r] = !edge || (k + r >= lo[mt] && k + r < hi[mt]) ? x : -INFINITY;
           }
+        c[u] = 1.f;
+        if (edge) {  // what no row sees may be anything
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (k + r < range.first || k + r >= range.end) {
+#pragma unroll
+              for (int j = 0; j < NV; ++j) vr[u][r][j] = 0u;
+            }
+          if (k + 3 < range.first || k >= range.end) w[u] = 0.f;
         }
-        if (k + 3 < range.first || k >= range.end) w[u] = 0.f;
       }
     }
-    const float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-    if (__any(top > m + kLazy)) {
-      const float m_new = fmaxf(m, row_groups_max(top));
-      const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+    // The largest logit of each row, from the products before their scale (scales are not negative).
+    float top[MT];
+    bool up = false;
 #pragma unroll
-      for (int n = 0; n < NO; ++n) acc[n] *= alpha;
-      l *= alpha;
-      m = m_new;
+    for (int mt = 0; mt < MT; ++mt) {
+      const float x0 = fmaxf(fmaxf(fmaxf(sa[mt][0][0], sa[mt][0][1]), sa[mt][0][2]), sa[mt][0][3]) * c[0];
+      const float x1 = fmaxf(fmaxf(fmaxf(sa[mt][1][0], sa[mt][1][1]), sa[mt][1][2]), sa[mt][1][3]) * c[1];
+      top[mt] = fmaxf(x0, x1);
+      up |= top[mt] > st.m[mt] + kLazy;
     }
-    float pv[8];
+    if (__any(up)) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int mt = 0; mt < MT; ++mt) {
+        const float m_new = fmaxf(st.m[mt], row_groups_max(top[mt]));
+        const float alpha = __builtin_amdgcn_exp2f(st.m[mt] - m_new);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float p = __builtin_amdgcn_exp2f(x[u][r] - m);
-        l += p;
-        pv[4 * u + r] = p * w[u];
+        for (int n = 0; n < NO; ++n) st.acc[mt][n] *= alpha;
+        st.l[mt] *= alpha;
+        st.m[mt] = m_new;
       }
-    bf16x8_t pf[kParts];
-    split<kParts>(pv, pf);
+    }
+    bf16x8_t pf[MT][kParts];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float pv[8];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(sa[mt][u][r], c[u], -st.m[mt]));
+          st.l[mt] += p;
+          pv[4 * u + r] = p * w[u];
+        }
+      split<kParts>(pv, pf[mt]);
+    }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       uint32_t pair[4][4];  // keys (0 1) (2 3) (16 17) (18 19) of the group, bytes 0..3
@@ -480,13 +486,53 @@ __device__ __forceinline__ void thin_item(const QuantArgs& a, const Seq& q, int 
       for (int b = 0; b < 4; ++b) {
         const bf16x8_t v = __builtin_bit_cast(bf16x8_t, u32x4_t{pair[0][b], pair[1][b], pair[2][b], pair[3][b]});
 #pragma unroll
-        for (int sp = 0; sp < kParts; ++sp) acc[4 * j + b] = mfma(v, pf[sp], acc[4 * j + b]);
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int sp = 0; sp < kParts; ++sp) st.acc[mt][4 * j + b] = mfma(v, pf[mt][sp], st.acc[mt][4 * j + b]);
       }
     }
-    if (more) load_v(k0 + 128, pg_next);
+    if (more) load_v(k0 + stride, pg_next);
     pg_next = pg_after;
   }
-  l = row_groups_sum(l);
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) st.l[mt] = row_groups_sum(st.l[mt]);
+}
+
+template <int D>
+struct ThinLds {
+  float o[4][4][D / 64][64][4];  // wavefront, r, piece, lane
+  float ml[4][16][2];
+};
+
+// A run of keys [ka, kb) (from the range's first key rounded down to 32) of one (sequence, kv head) with R <= 16 rows.
+// `self`: this workgroup's place in the cut; x0: the item's first position in the stream.
+template <int kCode, int D, typename T, int kParts, bool kCap>
+__device__ __forceinline__ void thin_item(Args& a, const Seq& q, int s, int h, int ka, int kb, const Cut& cut, int self, int64_t x0,
+                                          ThinLds<D>& lds, int* lds_flag) {
+  constexpr int NO = D / 16;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int G = a.group, R = q.q_len * G, dim = a.p.head_dim;
+  const Range range = key_range(a, q, 0, q.q_len);
+  const int base = range.first & ~31, keys = range.end - base;
+  const int token = i / G, head = h * G + i - token * G;
+  const bool real = i < R;
+  // keys of row i
+  const int pos = q.kv_len - q.q_len + token;
+  const int hi = real ? pos + 1 : 0;
+  const int lo = a.p.sliding_window > 0 ? max(static_cast<int>(max(static_cast<int64_t>(pos) - a.p.sliding_window + 1, static_cast<int64_t>(0))), 0) : 0;
+  const int full_lo = a.p.sliding_window > 0 ? max(q.kv_len - a.p.sliding_window, 0) : 0;  // keys every row sees
+  const int full_hi = q.kv_len - q.q_len + 1;
+
+  bf16x8_t qf[1][D / 32][kParts];
+  {
+    const T* row = static_cast<const T*>(a.p.queries) + (q.q0 + (real ? token : 0)) * a.p.query_token_stride + (real ? head : 0) * a.p.query_head_stride;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) load_q<T, kParts>(row, real, 16 * (g + 4 * (k >> 1)) + 8 * (k & 1), dim, qf[0][k]);
+  }
+  RowState<1, D> st;
+  walk<kCode, D, kParts, kCap, 1>(a, q, s, h, qf, {lo}, {hi}, range, full_lo, full_hi, base + ka + 32 * wave, base + ((min(kb, keys) + 31) & ~31), 128, st);
+  const auto& acc = st.acc[0];
+  const float m = st.m[0], l = st.l[0];
 
   // The four wavefronts meet: wavefront w adds up outputs NO (4 g + w) .. + NO of every row.
   __syncthreads();  // LDS may hold what came before
@@ -565,12 +611,11 @@ struct TileLds {
 
 // A run of keys [ka, kb) of one tile of rows.
 template <int kCode, int D, typename T, int kParts, bool kCap>
-__device__ __forceinline__ void tile_item(const QuantArgs& a, const Seq& q, int s, int hs, int tile, int ka, int kb, const Cut& cut, int self, int64_t x0,
-                                          char* lds_raw, int* lds_flag) {
+__device__ __forceinline__ void tile_item(Args& a, const Seq& q, int s, int hs, int tile, int ka, int kb, const Cut& cut, int self, int64_t x0,
+                                          TileLds<D>& lds, int* lds_flag) {
   constexpr int kStep = quant_step_keys<D>(), kRowTiles = quant_row_tiles<D, kParts>();
   constexpr int NP = D / 64, NO = D / 16, kSub = kStep / 16, kBlocks = kStep / 32;
   constexpr int kUnitsK = kSub * NP / 4, kUnitsV = (kBlocks * NP + 3) / 4;  // per wavefront
-  TileLds<D>& lds = *reinterpret_cast<TileLds<D>*>(lds_raw);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
   const int dim = a.p.head_dim;
   const int h = hs / a.subs, sub = hs - h * a.subs;
@@ -611,16 +656,21 @@ __device__ __forceinline__ void tile_item(const QuantArgs& a, const Seq& q, int 
   const int last_page = max(q.kv_len - 1, 0) >> a.page_shift;
   u32x4_t kr[kUnitsK];
   uint32_t vr[kUnitsV][2][4];
-  float sc = 0.f;
-  int scale_key = 0;
+  float k_scale = 0.f, v_scale = 0.f;  // of four keys of the step, the first lanes of wavefront 0
   // K unit x: 16 keys, 16 elements a lane; V unit x: 32 keys (8 a lane), 64 elements (4 a lane)
-  auto load_codes = [&](int k0) {
+  auto load_k = [&](int k0) {
 #pragma unroll
     for (int n = 0; n < kUnitsK; ++n) {
       const int x = wave * kUnitsK + n, u = x / NP, piece = g + 4 * (x % NP);
       const int k = k0 + 16 * u + i;
       kr[n] = *reinterpret_cast<const u32x4_t*>(row_of(a, page_of_key(a, table, k, last_page), 2 * h, k) + (16 * piece < dim ? 16 * piece : 0));
     }
+    if (threadIdx.x < kStep / 4) {
+      const int k = k0 + 4 * threadIdx.x;
+      k_scale = *scale_of(a, page_of_key(a, table, k, last_page), 2 * h, k);
+    }
+  };
+  auto load_v = [&](int k0) {
 #pragma unroll
     for (int n = 0; n < kUnitsV; ++n) {
       const int x = (wave * kUnitsV + n) % (kBlocks * NP), b = x / NP, d = 64 * (x % NP) + 4 * i;
@@ -632,16 +682,15 @@ __device__ __forceinline__ void tile_item(const QuantArgs& a, const Seq& q, int 
         for (int r = 0; r < 4; ++r) vr[n][u][r] = *reinterpret_cast<const uint32_t*>(row + r * dim);
       }
     }
-    if (threadIdx.x < kStep / 2) {  // groups of 4 keys: the scales of K, then of V
-      const int half = threadIdx.x / (kStep / 4), k = k0 + 4 * (threadIdx.x - half * (kStep / 4));
-      sc = *scale_of(a, page_of_key(a, table, k, last_page), 2 * h + half, k);
-      scale_key = k;
+    if (threadIdx.x < kStep / 4) {
+      const int k = k0 + 4 * threadIdx.x;
+      v_scale = *scale_of(a, page_of_key(a, table, k, last_page), 2 * h + 1, k);
     }
   };
   const float cap = a.p.logits_soft_cap, inv_cap = kCap ? 1.f / cap : 0.f;
   const float c_scale = kCap ? a.p.softmax_scale : a.p.softmax_scale * kLog2e, cap2 = cap * kLog2e;
-  auto store_codes = [&](int k0, int buf) {
-    const bool edge = k0 < range.first || k0 + kStep > range.end;
+  auto in_range = [&](int k, int n) { return k + n > range.first && k < range.end; };  // any of n keys from k on
+  auto store_k = [&](int k0, int buf) {
 #pragma unroll
     for (int n = 0; n < kUnitsK; ++n) {
       const int x = wave * kUnitsK + n, u = x / NP, np = x % NP;
@@ -650,6 +699,10 @@ __device__ __forceinline__ void tile_item(const QuantArgs& a, const Seq& q, int 
       lds.k[buf][u][2 * np][lane] = op[0];
       lds.k[buf][u][2 * np + 1][lane] = op[1];
     }
+    if (threadIdx.x < kStep / 4) lds.ks[buf][threadIdx.x] = in_range(k0 + 4 * threadIdx.x, 4) ? k_scale * c_scale : 0.f;
+  };
+  auto store_v = [&](int k0, int buf) {
+    const bool edge = k0 < range.first || k0 + kStep > range.end;
 #pragma unroll
     for (int n = 0; n < kUnitsV; ++n) {
       const int x = wave * kUnitsV + n, b = x / NP, j = x % NP;
@@ -658,10 +711,7 @@ __device__ __forceinline__ void tile_item(const QuantArgs& a, const Seq& q, int 
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int k = k0 + 32 * b + 16 * u + 4 * g + r;
-            if (k < range.first || k >= range.end) vr[n][u][r] = 0u;
-          }
+          for (int r = 0; r < 4; ++r) vr[n][u][r] = in_range(k0 + 32 * b + 16 * u + 4 * g + r, 1) ? vr[n][u][r] : 0u;
       }
       uint32_t pair[4][4];
 #pragma unroll
@@ -673,89 +723,141 @@ __device__ __forceinline__ void tile_item(const QuantArgs& a, const Seq& q, int 
       for (int e = 0; e < 4; ++e)
         lds.v[buf][b][4 * j + e][lane] = __builtin_bit_cast(bf16x8_t, u32x4_t{pair[0][e], pair[1][e], pair[2][e], pair[3][e]});
     }
-    if (threadIdx.x < kStep / 2) {
-      float y = sc;
-      if (scale_key + 3 < range.first || scale_key >= range.end) y = 0.f;
-      float* dst = threadIdx.x < kStep / 4 ? lds.ks[buf] + threadIdx.x : lds.vs[buf] + threadIdx.x - kStep / 4;
-      *dst = threadIdx.x < kStep / 4 ? y * c_scale : y;
-    }
+    if (threadIdx.x < kStep / 4) lds.vs[buf][threadIdx.x] = in_range(k0 + 4 * threadIdx.x, 4) ? v_scale : 0.f;
   };
-
-  const int t_begin = ka / kStep, t_end = (min(kb, keys) + kStep - 1) / kStep;
-  __syncthreads();  // LDS may hold what came before
-  if (t_begin < t_end) {
-    load_codes(base + t_begin * kStep);
-    store_codes(base + t_begin * kStep, 0);
-    if (t_begin + 1 < t_end) load_codes(base + (t_begin + 1) * kStep);
-  }
-  for (int t = t_begin; t < t_end; ++t) {
-    const int k0 = base + t * kStep, buf = (t - t_begin) & 1;
-    __syncthreads();
-    const bool edge = k0 < full_lo || k0 + kStep > full_hi;
+  // The loop is a pipeline of two stages, so that the matrix unit always has work beside the vector unit's: while the
+  // probabilities of step t are taken, the logits of step t + 1 are multiplied; while the outputs of step t are
+  // multiplied, the codes of K of step t + 2 and of V of step t + 1 are widened into LDS.  One barrier a step: K (t + 2)
+  // replaces K (t), whose last reads lie before the barrier, and V (t + 1) replaces V (t - 1), likewise.
+  typedef f32x4_t Scores[kRowTiles][kSub];
+  auto multiply_k = [&](Scores& sa, int buf) {
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-      f32x4_t sa[kRowTiles][2];
+    for (int u = 0; u < kSub; ++u) {
 #pragma unroll
-      for (int mt = 0; mt < kRowTiles; ++mt) sa[mt][0] = sa[mt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int mt = 0; mt < kRowTiles; ++mt) sa[mt][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
-          const bf16x8_t op = lds.k[buf][2 * b + u][k][lane];
-#pragma unroll
-          for (int mt = 0; mt < kRowTiles; ++mt)
-#pragma unroll
-            for (int sp = 0; sp < kParts; ++sp) sa[mt][u] = mfma(op, qf[mt][k][sp], sa[mt][u]);
-        }
-      bf16x8_t pf[kRowTiles][kParts];
-      const float c[2] = {lds.ks[buf][8 * b + g], lds.ks[buf][8 * b + 4 + g]}, w[2] = {lds.vs[buf][8 * b + g], lds.vs[buf][8 * b + 4 + g]};
-#pragma unroll
-      for (int mt = 0; mt < kRowTiles; ++mt) {
-        float x[2][4];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) x[u][r] = scaled<kCap>(sa[mt][u][r], c[u], cap2, inv_cap);
-        if (edge) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int k = k0 + 32 * b + 16 * u + 4 * g + r;
-              x[u][r] = k >= lo[mt] && k < hi[mt] ? x[u][r] : -INFINITY;
-            }
-        }
-        const float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-        if (__any(top > m[mt] + kLazy)) {
-          const float m_new = fmaxf(m[mt], row_groups_max(top));
-          const float alpha = __builtin_amdgcn_exp2f(m[mt] - m_new);
-#pragma unroll
-          for (int n = 0; n < NO; ++n) acc[mt][n] *= alpha;
-          l[mt] *= alpha;
-          m[mt] = m_new;
-        }
-        float pv[8];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float p = __builtin_amdgcn_exp2f(x[u][r] - m[mt]);
-            l[mt] += p;
-            pv[4 * u + r] = p * w[u];
-          }
-        split<kParts>(pv, pf[mt]);
-      }
-      if (b == kBlocks - 1 && t + 1 < t_end) {  // the next step's codes have come in meanwhile
-        store_codes(k0 + kStep, buf ^ 1);
-        if (t + 2 < t_end) load_codes(k0 + 2 * kStep);
-      }
-#pragma unroll
-      for (int n = 0; n < NO; ++n) {
-        const bf16x8_t v = lds.v[buf][b][n][lane];
+      for (int k = 0; k < D / 32; ++k) {
+        const bf16x8_t op = lds.k[buf][u][k][lane];
 #pragma unroll
         for (int mt = 0; mt < kRowTiles; ++mt)
 #pragma unroll
-          for (int sp = 0; sp < kParts; ++sp) acc[mt][n] = mfma(v, pf[mt][sp], acc[mt][n]);
+          for (int sp = 0; sp < kParts; ++sp) sa[mt][u] = mfma(op, qf[mt][k][sp], sa[mt][u]);
+      }
+    }
+  };
+  // Scales (not negative), cap and mask of a step's logits, and the running maximum's move.  c: what is left to multiply by.
+  auto prepare = [&](Scores& sa, float (&c)[kSub], int k0, int buf) {
+#pragma unroll
+    for (int u = 0; u < kSub; ++u) c[u] = lds.ks[buf][4 * u + g];
+    const bool edge = k0 < full_lo || k0 + kStep > full_hi;
+    if (kCap || edge) {
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) {
+#pragma unroll
+        for (int mt = 0; mt < kRowTiles; ++mt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int k = k0 + 16 * u + 4 * g + r;
+            const float x = scaled<kCap>(sa[mt][u][r], c[u], cap2, inv_cap);
+            sa[mt][u][r] = !edge || (k >= lo[mt] && k < hi[mt]) ? x : -INFINITY;
+          }
+        c[u] = 1.f;
+      }
+    }
+    float top[kRowTiles];
+    bool up = false;
+#pragma unroll
+    for (int mt = 0; mt < kRowTiles; ++mt) {
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) {
+        const float x = fmaxf(fmaxf(fmaxf(sa[mt][u][0], sa[mt][u][1]), sa[mt][u][2]), sa[mt][u][3]) * c[u];
+        top[mt] = u == 0 ? x : fmaxf(top[mt], x);
+      }
+      up |= top[mt] > m[mt] + kLazy;
+    }
+    if (__any(up)) {
+#pragma unroll
+      for (int mt = 0; mt < kRowTiles; ++mt) {
+        const float m_new = fmaxf(m[mt], row_groups_max(top[mt]));
+        const float alpha = __builtin_amdgcn_exp2f(m[mt] - m_new);
+#pragma unroll
+        for (int n = 0; n < NO; ++n) acc[mt][n] *= alpha;
+        l[mt] *= alpha;
+        m[mt] = m_new;
+      }
+    }
+  };
+  auto probabilities = [&](const Scores& sa, const float (&c)[kSub], int buf, bf16x8_t (&pf)[kBlocks][kRowTiles][kParts]) {
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+      for (int mt = 0; mt < kRowTiles; ++mt) {
+        float pv[8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float w = lds.vs[buf][8 * b + 4 * u + g];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(sa[mt][2 * b + u][r], c[2 * b + u], -m[mt]));
+            l[mt] += p;
+            pv[4 * u + r] = p * w;
+          }
+        }
+        split<kParts>(pv, pf[b][mt]);
+      }
+  };
+
+  const int t_begin = ka / kStep, t_end = (min(kb, keys) + kStep - 1) / kStep;
+  auto key_of = [&](int t) { return base + t * kStep; };
+  __syncthreads();  // LDS may hold what came before
+  if (t_begin < t_end) {
+    Scores sa;
+    float c[kSub];
+    load_k(key_of(t_begin));
+    load_v(key_of(t_begin));
+    store_k(key_of(t_begin), 0);
+    if (t_begin + 1 < t_end) load_k(key_of(t_begin + 1));
+    store_v(key_of(t_begin), 0);
+    if (t_begin + 1 < t_end) {
+      load_v(key_of(t_begin + 1));
+      store_k(key_of(t_begin + 1), 1);
+      if (t_begin + 2 < t_end) load_k(key_of(t_begin + 2));
+    }
+    __syncthreads();
+    multiply_k(sa, 0);
+    prepare(sa, c, key_of(t_begin), 0);
+    for (int t = t_begin; t < t_end; ++t) {
+      const int buf = (t - t_begin) & 1;
+      if (t > t_begin) __syncthreads();
+      const bool more = t + 1 < t_end;
+      Scores sb;
+      bf16x8_t pf[kBlocks][kRowTiles][kParts];
+      if (more) multiply_k(sb, buf ^ 1);
+      probabilities(sa, c, buf, pf);
+      if (more) {
+        if (t + 2 < t_end) {
+          store_k(key_of(t + 2), buf);
+          if (t + 3 < t_end) load_k(key_of(t + 3));
+        }
+        store_v(key_of(t + 1), buf ^ 1);
+        if (t + 2 < t_end) load_v(key_of(t + 2));
+      }
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int n = 0; n < NO; ++n) {
+          const bf16x8_t v = lds.v[buf][b][n][lane];
+#pragma unroll
+          for (int mt = 0; mt < kRowTiles; ++mt)
+#pragma unroll
+            for (int sp = 0; sp < kParts; ++sp) acc[mt][n] = mfma(v, pf[b][mt][sp], acc[mt][n]);
+        }
+      if (more) {
+        prepare(sb, c, key_of(t + 1), buf ^ 1);
+#pragma unroll
+        for (int mt = 0; mt < kRowTiles; ++mt)
+#pragma unroll
+          for (int u = 0; u < kSub; ++u) sa[mt][u] = sb[mt][u];
       }
     }
   }
@@ -823,156 +925,183 @@ __device__ __forceinline__ int place_in_cut(int b, int n) {
   return j < per + (xcd < rem ? 1 : 0) ? xcd * per + min(xcd, rem) + j : -1;
 }
 
+// A workgroup's run of a stream: [x, x_end) of `cut`, beginning `off` positions into sequence `seq` of n.
+struct Run {
+  Cut cut;
+  int self, seq, n;
+  int64_t x, x_end, off;
+};
+
 struct SchedLds {
   int64_t sums[4][2];
-  int longest[4];
-  int items[4];
-  int seq[2];
-  int64_t off[2];
+  Run run[2];
   int flag;
 };
 
+template <int D>
+struct Lds {
+  union {
+    ThinLds<D> thin;
+    TileLds<D> tile;
+  };
+  SchedLds sched;
+};
+template <int D>
+__device__ __forceinline__ Lds<D>& lds_of() {
+  __shared__ __align__(16) char bytes[sizeof(Lds<D>)];
+  return *reinterpret_cast<Lds<D>*>(bytes);
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(x)), hi = __builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32));
+  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ Run uniform(const Run& r) {
+  return {{uniform(r.cut.total), uniform(r.cut.n)}, uniform(r.self), uniform(r.seq), uniform(r.n), uniform(r.x), uniform(r.x_end), uniform(r.off)};
+}
+
+// The two streams are functions of their own, so that the registers of one loop are not shared out by the other's.
 template <int kCode, int D, typename T, int kParts, bool kCap>
-__global__ __launch_bounds__(256, 2) void quant_attention_kernel(QuantArgs a) {
-  constexpr size_t kLds = sizeof(TileLds<D>) > sizeof(ThinLds<D>) ? sizeof(TileLds<D>) : sizeof(ThinLds<D>);
-  __shared__ __align__(16) char lds[kLds];
-  __shared__ SchedLds sched;
+__device__ __attribute__((noinline)) void thin_phase(uint64_t args) {
+  Args& a = *reinterpret_cast<Args*>(uniform(static_cast<int64_t>(args)));
+  Lds<D>& lds = lds_of<D>();
+  const Run run = uniform(lds.sched.run[0]);
+  Window window;
+  int s = run.seq;
+  int64_t off = run.off, x = run.x;
+  while (x < run.x_end && s < run.n) {
+    window.at(a, run.n, s);
+    const Seq q = window.get(s);
+    const int keys = thin_keys(a, q), len = keys + kThinPad;
+    const Range range = key_range(a, q, 0, q.q_len);
+    const int all = range.end - (range.first & ~31);  // keys as they are walked
+    int h = static_cast<int>(off / len);
+    int begin = static_cast<int>(off - static_cast<int64_t>(h) * len);
+    for (; h < a.p.num_kv_heads && x < run.x_end; ++h, begin = 0) {
+      const int end = static_cast<int>(min(static_cast<int64_t>(len), begin + (run.x_end - x)));
+      const int ka = begin >= keys ? all : begin / kThinStep * kThinStep, kb = end >= keys ? all : end / kThinStep * kThinStep;
+      if (ka < kb || (keys == 0 && begin == 0))
+        thin_item<kCode, D, T, kParts, kCap>(a, q, s, h, keys == 0 ? 0 : ka, kb, run.cut, run.self, x - begin, lds.thin, &lds.sched.flag);
+      x += end - begin;
+    }
+    off = 0;
+    s = window.next(a, run.n, s + 1, true);
+  }
+}
+
+template <int kCode, int D, typename T, int kParts, bool kCap>
+__device__ __attribute__((noinline)) void tile_phase(uint64_t args) {
+  constexpr int kStep = quant_step_keys<D>();
+  Args& a = *reinterpret_cast<Args*>(uniform(static_cast<int64_t>(args)));
+  Lds<D>& lds = lds_of<D>();
+  const Run run = uniform(lds.sched.run[1]);
+  Window window;
+  int s = run.seq;
+  int64_t off = run.off, x = run.x;
+  const int heads = a.p.num_kv_heads * a.subs;
+  while (x < run.x_end && s < run.n) {
+    window.at(a, run.n, s);
+    const Seq q = window.get(s);
+    const int tiles = tiles_of(a, q);
+    const int64_t len = tiles_before(a, q, tiles, true);
+    int h = static_cast<int>(off / len);
+    int64_t rest = off - static_cast<int64_t>(h) * len;
+    int tile = 0;
+    for (int hi = tiles; hi - tile > 1;) {  // the last tile that starts at or before the position
+      const int mid = (tile + hi) >> 1;
+      if (tiles_before(a, q, mid, false) <= rest) tile = mid;
+      else hi = mid;
+    }
+    int begin = static_cast<int>(rest - tiles_before(a, q, tile, false));
+    for (; h < heads && x < run.x_end; ++h, tile = 0) {
+      for (; tile < tiles && x < run.x_end; ++tile, begin = 0) {
+        const Range range = key_range(a, q, tile * a.tile_tokens, min((tile + 1) * a.tile_tokens, q.q_len));
+        const int keys = range.end - range.first, all = range.end - (range.first & ~31), item = keys + kTilePad;
+        const int end = static_cast<int>(min(static_cast<int64_t>(item), begin + (run.x_end - x)));
+        const int ka = begin >= keys ? all : begin / kStep * kStep, kb = end >= keys ? all : end / kStep * kStep;
+        if (ka < kb || (keys == 0 && begin == 0))
+          tile_item<kCode, D, T, kParts, kCap>(a, q, s, h, tile, keys == 0 ? 0 : ka, kb, run.cut, run.self, x - begin, lds.tile, &lds.sched.flag);
+        x += end - begin;
+      }
+    }
+    off = 0;
+    s = window.next(a, run.n, s + 1, false);
+  }
+}
+
+template <int kCode, int D, typename T, int kParts, bool kCap>
+__global__ __launch_bounds__(256, 2) void quant_attention_kernel(QuantArgs) {
+  Args& a = *(Args*)__builtin_amdgcn_kernarg_segment_ptr();
+  SchedLds& sched = lds_of<D>().sched;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n = min(max(a.p.num_seqs[0], 0), a.p.max_num_seqs);
-  const int heads[2] = {a.p.num_kv_heads, a.p.num_kv_heads * a.subs};
 
-  // Lengths of the two streams, and the longest item and the number of items of the first.
+  // Lengths of the two streams.
   const int per = (n + 255) >> 8;
   const int s0 = min(static_cast<int>(threadIdx.x) * per, n), s1 = min(s0 + per, n);
+  auto length = [&](const Seq& q, bool thin) {
+    return thin ? static_cast<int64_t>(thin_keys(a, q) + kThinPad) * a.p.num_kv_heads : tiles_before(a, q, tiles_of(a, q), true) * a.p.num_kv_heads * a.subs;
+  };
   int64_t sum[2] = {0, 0};
-  int longest = 0, items = 0;
   for (int s = s0; s < s1; ++s) {
     const Seq q = load_seq(a, n, s);
     if (q.q_len == 0) continue;
-    if (is_thin(a, q)) {
-      const int k = thin_keys(a, q);
-      sum[0] += static_cast<int64_t>(k + kThinPad) * heads[0];
-      longest = max(longest, k);
-      items += heads[0];
-    } else {
-      sum[1] += tiles_before(a, q, tiles_of(a, q), true) * heads[1];
-    }
+    const bool thin = is_thin(a, q);
+    sum[thin ? 0 : 1] += length(q, thin);
   }
   int64_t inc[2] = {sum[0], sum[1]};
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const int64_t x = __shfl_up(inc[0], o), y = __shfl_up(inc[1], o);
     if (lane >= o) inc[0] += x, inc[1] += y;
-    longest = max(longest, __shfl_xor(longest, o));
-    items += __shfl_xor(items, o);
   }
-  if (lane == 63) {
-    sched.sums[wave][0] = inc[0], sched.sums[wave][1] = inc[1];
-    sched.longest[wave] = longest, sched.items[wave] = items;
-  }
+  if (lane == 63) sched.sums[wave][0] = inc[0], sched.sums[wave][1] = inc[1];
   __syncthreads();
   int64_t before[2] = {inc[0] - sum[0], inc[1] - sum[1]}, total[2] = {0, 0};
-  longest = items = 0;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
     if (w < wave) before[0] += sched.sums[w][0], before[1] += sched.sums[w][1];
     total[0] += sched.sums[w][0], total[1] += sched.sums[w][1];
-    longest = max(longest, sched.longest[w]);
-    items += sched.items[w];
   }
-  Cut cut[2];
-  cut[0].total = total[0];
-  cut[0].n = static_cast<int>(min(static_cast<int64_t>(a.grid), max(total[0] / kThinLeast, static_cast<int64_t>(1))));
-  cut[1].total = total[1];
-  cut[1].n = static_cast<int>(min(static_cast<int64_t>(a.grid), max(total[1] / kTileLeast, static_cast<int64_t>(1))));
-  // the first stream from the grid's front, the second from its back: where both are short they meet different workgroups
-  const int mine[2] = {total[0] > 0 ? place_in_cut(blockIdx.x, cut[0].n) : -1, total[1] > 0 ? place_in_cut(a.grid - 1 - blockIdx.x, cut[1].n) : -1};
-  int64_t x_begin[2] = {0, 0}, x_end[2] = {0, 0};
-#pragma unroll
-  for (int c = 0; c < 2; ++c)
-    if (mine[c] >= 0) x_begin[c] = cut[c].bound(mine[c]), x_end[c] = cut[c].bound(mine[c] + 1);
-  // the thread whose sequences hold a run's first position finds it
+  bool has[2];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    if (mine[c] < 0 || x_begin[c] < before[c] || x_begin[c] >= before[c] + sum[c]) continue;
-    int64_t off = x_begin[c] - before[c];
-    for (int s = s0; s < s1; ++s) {
-      const Seq q = load_seq(a, n, s);
-      if (q.q_len == 0 || is_thin(a, q) != (c == 0)) continue;
-      const int64_t len = c == 0 ? static_cast<int64_t>(thin_keys(a, q) + kThinPad) * heads[0] : tiles_before(a, q, tiles_of(a, q), true) * heads[1];
-      if (off < len) {
-        sched.seq[c] = s;
-        sched.off[c] = off;
-        break;
+    Run r;
+    r.seq = 0, r.off = 0;
+    r.n = n;
+    r.cut.total = total[c];
+    r.cut.n = static_cast<int>(min(static_cast<int64_t>(a.grid), max(total[c] / (c == 0 ? kThinLeast : kTileLeast), static_cast<int64_t>(1))));
+    // the first stream from the grid's front, the second from its back: where both are short they meet different workgroups
+    r.self = total[c] > 0 ? place_in_cut(c == 0 ? blockIdx.x : a.grid - 1 - blockIdx.x, r.cut.n) : -1;
+    r.x = r.self >= 0 ? r.cut.bound(r.self) : 0;
+    r.x_end = r.self >= 0 ? r.cut.bound(r.self + 1) : 0;
+    has[c] = r.x < r.x_end;
+    // the thread whose sequences hold the run's first position finds it
+    if (r.self >= 0 && r.x >= before[c] && r.x < before[c] + sum[c]) {
+      int64_t off = r.x - before[c];
+      for (int s = s0; s < s1; ++s) {
+        const Seq q = load_seq(a, n, s);
+        if (q.q_len == 0 || is_thin(a, q) != (c == 0)) continue;
+        const int64_t len = length(q, c == 0);
+        if (off < len) {
+          r.seq = s;
+          r.off = off;
+          sched.run[c] = r;
+          break;
+        }
+        off -= len;
       }
-      off -= len;
     }
   }
   __syncthreads();
-
-  Window window;
-  auto thin_phase = [&] {
-    if (x_begin[0] >= x_end[0]) return;
-    int s = __builtin_amdgcn_readfirstlane(sched.seq[0]);
-    int64_t off = sched.off[0], x = x_begin[0];
-    while (x < x_end[0] && s < n) {
-      window.at(a, n, s);
-      const Seq q = window.get(s);
-      const int keys = thin_keys(a, q), len = keys + kThinPad;
-      const Range range = key_range(a, q, 0, q.q_len);
-      const int all = range.end - (range.first & ~31);  // keys as they are walked
-      int h = static_cast<int>(off / len);
-      int begin = static_cast<int>(off - static_cast<int64_t>(h) * len);
-      for (; h < heads[0] && x < x_end[0]; ++h, begin = 0) {
-        const int end = static_cast<int>(min(static_cast<int64_t>(len), begin + (x_end[0] - x)));
-        const int ka = begin >= keys ? all : begin / kThinStep * kThinStep, kb = end >= keys ? all : end / kThinStep * kThinStep;
-        if (ka < kb || (keys == 0 && begin == 0))
-          thin_item<kCode, D, T, kParts, kCap>(a, q, s, h, keys == 0 ? 0 : ka, kb, cut[0], mine[0], x - begin, lds, &sched.flag);
-        x += end - begin;
-      }
-      off = 0;
-      s = window.next(a, n, s + 1, true);
-    }
-  };
-  auto tile_phase = [&] {
-    if (x_begin[1] >= x_end[1]) return;
-    constexpr int kStep = quant_step_keys<D>();
-    int s = __builtin_amdgcn_readfirstlane(sched.seq[1]);
-    int64_t off = sched.off[1], x = x_begin[1];
-    while (x < x_end[1] && s < n) {
-      window.at(a, n, s);
-      const Seq q = window.get(s);
-      const int tiles = tiles_of(a, q);
-      const int64_t len = tiles_before(a, q, tiles, true);
-      int h = static_cast<int>(off / len);
-      int64_t rest = off - static_cast<int64_t>(h) * len;
-      int tile = 0;
-      for (int hi = tiles; hi - tile > 1;) {  // the last tile that starts at or before the position
-        const int mid = (tile + hi) >> 1;
-        if (tiles_before(a, q, mid, false) <= rest) tile = mid;
-        else hi = mid;
-      }
-      int begin = static_cast<int>(rest - tiles_before(a, q, tile, false));
-      for (; h < heads[1] && x < x_end[1]; ++h, tile = 0) {
-        for (; tile < tiles && x < x_end[1]; ++tile, begin = 0) {
-          const Range range = key_range(a, q, tile * a.tile_tokens, min((tile + 1) * a.tile_tokens, q.q_len));
-          const int keys = range.end - range.first, all = range.end - (range.first & ~31), item = keys + kTilePad;
-          const int end = static_cast<int>(min(static_cast<int64_t>(item), begin + (x_end[1] - x)));
-          const int ka = begin >= keys ? all : begin / kStep * kStep, kb = end >= keys ? all : end / kStep * kStep;
-          if (ka < kb || (keys == 0 && begin == 0))
-            tile_item<kCode, D, T, kParts, kCap>(a, q, s, h, tile, keys == 0 ? 0 : ka, kb, cut[1], mine[1], x - begin, lds, &sched.flag);
-          x += end - begin;
-        }
-      }
-      off = 0;
-      s = window.next(a, n, s + 1, false);
-    }
-  };
   const bool thin_first = static_cast<int>(blockIdx.x) * 2 < a.grid;
 #pragma unroll 1
   for (int k = 0; k < 2; ++k) {
-    if ((k == 0) == thin_first) thin_phase();
-    else tile_phase();
+    const int c = (k == 0) == thin_first ? 0 : 1;
+    const uint64_t args = reinterpret_cast<uint64_t>(&a);
+    if (c == 0 && has[0]) thin_phase<kCode, D, T, kParts, kCap>(args);
+    if (c == 1 && has[1]) tile_phase<kCode, D, T, kParts, kCap>(args);
   }
 
   // Rows in front of the first sequence and behind the last are zeros.
