@@ -43,6 +43,8 @@ int check_attention(const RpaQuantParams& p) {
     return fail(RPA_ERR_INVALID_ARGUMENT, "non-positive dimension in RpaQuantParams");
   if (p.num_q_heads % p.num_kv_heads != 0)
     return fail(RPA_ERR_INVALID_ARGUMENT, "num_q_heads=%d must be divisible by num_kv_heads=%d", p.num_q_heads, p.num_kv_heads);
+  if (static_cast<int64_t>(p.pages_per_seq) * p.page_size > (1 << 30))
+    return fail(RPA_ERR_UNSUPPORTED, "pages_per_seq * page_size = %lld: a sequence holds at most 2^30 tokens", static_cast<long long>(p.pages_per_seq) * p.page_size);
   if (p.sliding_window < 0) return fail(RPA_ERR_INVALID_ARGUMENT, "sliding_window=%d must be positive", p.sliding_window);
   if (!std::isfinite(p.softmax_scale)) return fail(RPA_ERR_INVALID_ARGUMENT, "softmax_scale must be finite");
   if (!std::isfinite(p.logits_soft_cap)) return fail(RPA_ERR_INVALID_ARGUMENT, "logits_soft_cap must be finite");

@@ -41,10 +41,9 @@ struct QuantArgs {
 };
 
 // Shape of the second stream's tiles for a (padded) head_dim: keys per step, and 16-row tiles per wavefront.
-template <int D>
-constexpr int quant_step_keys() { return D == 256 ? 32 : 64; }
 template <int D, int kParts>
-constexpr int quant_row_tiles() { return kParts == 3 || D == 256 ? 1 : 2; }
+constexpr int quant_row_tiles() { return kParts == 3 || D == 256 ? 1 : 3; }
+constexpr int kTileStep = 32;
 
 constexpr int kThinStep = 128;     // keys a workgroup takes at once in the first stream
 constexpr int kThinPad = 128;      // what an item of the first stream costs beyond its keys, in keys
@@ -145,17 +144,15 @@ struct Window {
   }
 };
 
-// First key row of (page of key k, combined head) in the pool, in rows of the head's page.
-__device__ __forceinline__ int page_of_key(Args& a, const int32_t* __restrict__ table, int k, int last_page) {
-  return clamp_page(table[min(k >> a.page_shift, last_page)], a.p.num_pages);
-}
+// Row of key k of a combined head, and its block's scale, in the page that the block table names (clamped here, where it is
+// used, so that nothing waits for it where it is loaded).
 __device__ __forceinline__ const char* row_of(Args& a, int page, int head, int k) {
-  const uint64_t line = static_cast<uint64_t>(page) * (2 * a.p.num_kv_heads) + head;
+  const uint64_t line = static_cast<uint64_t>(clamp_page(page, a.p.num_pages)) * (2 * a.p.num_kv_heads) + head;
   const uint64_t row = (line << a.page_shift) + (k & ((1 << a.page_shift) - 1));
   return static_cast<const char*>(a.p.kv_cache) + row * a.p.head_dim;
 }
 __device__ __forceinline__ const float* scale_of(Args& a, int page, int head, int k) {
-  const uint64_t line = static_cast<uint64_t>(page) * (2 * a.p.num_kv_heads) + head;
+  const uint64_t line = static_cast<uint64_t>(clamp_page(page, a.p.num_pages)) * (2 * a.p.num_kv_heads) + head;
   return a.p.kv_scales + (line << (a.page_shift - a.block_shift)) + ((k & ((1 << a.page_shift) - 1)) >> a.block_shift);
 }
 
@@ -224,6 +221,16 @@ __device__ __forceinline__ void widen_pairs(uint32_t x, uint32_t y, uint32_t (&p
     pair[3] = codes_to_bf16<kCode, true>(hi);
   }
 }
+
+// Loads on either side stay there: they are counted as they come in, so one that the compiler moves behind the others
+// waits for all of them.
+// A lane offset as it stands beside its load, where the load takes it with a scalar base (hoisted, it becomes a pair of
+// registers that is added to the base for every load).
+__device__ __forceinline__ uint32_t here(uint32_t off) {
+  asm volatile("" : "+v"(off));
+  return off;
+}
+__device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
 
 __device__ __forceinline__ f32x4_t mfma(bf16x8_t a, bf16x8_t b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
@@ -315,8 +322,8 @@ struct RowState {
   f32x4_t acc[MT][kD / 16];  // output element (kD / 16) (4 g + r) + n of row i, unnormalised
   float m[MT], l[MT];        // running maximum (log2) of the row, this lane's share of its sum
 };
-template <int kCode, int D, int kParts, bool kCap, int MT>
-__device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const bf16x8_t (&qf)[MT][D / 32][kParts], const int (&lo)[MT],
+template <int kCode, int D, int kParts, bool kCap, bool kWide, int MT>
+__device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const bf16x8_t (&qf)[MT][D / 32][kParts],
                                      const int (&hi)[MT], const Range& range, int full_lo, int full_hi, int k_begin, int k_end, int stride,
                                      RowState<MT, D>& st) {
   constexpr int NP = D / 64, NV = D / 64, NO = D / 16;
@@ -330,21 +337,30 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
   if (k_begin >= k_end) return;
   const int32_t* __restrict__ table = a.p.block_tables + static_cast<size_t>(s) * a.p.pages_per_seq;
   const int last_page = max(q.kv_len - 1, 0) >> a.page_shift;
-  // pieces beyond head_dim read the row's first again (the queries are zero there, the outputs not stored)
-  int k_off[NP];
+  // Lane offsets inside 16 keys of a head.  Pieces beyond head_dim read the row's first again (the queries are zero there,
+  // the outputs not stored).
+  uint32_t k_off[NP], v_off[4];
 #pragma unroll
-  for (int n = 0; n < NP; ++n) k_off[n] = 16 * (g + 4 * n) < dim ? 16 * (g + 4 * n) : 0;
-  const int v_off = NO * i < dim ? NO * i : 0;
+  for (int n = 0; n < NP; ++n) k_off[n] = (kWide ? i * dim : 0) + (16 * (g + 4 * n) < dim ? 16 * (g + 4 * n) : 0);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v_off[r] = ((kWide ? 4 * g : 0) + r) * dim + (NO * i < dim ? NO * i : 0);
+  const uint32_t sc_off = 4 * g >> a.block_shift;
 
+  // Pages of 16 tokens and more (kWide): 16 keys have one page, whose address is scalar.  Shorter ones: a page for each
+  // lane's key of K and for each lane's four keys of V.
   struct Pages {
-    int k[2], v[2];
+    int k[2] = {0, 0}, v[2] = {0, 0};
   };
   auto load_pages = [&](int k0) {
     Pages pg;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      pg.k[u] = page_of_key(a, table, k0 + 16 * u + i, last_page);
-      pg.v[u] = page_of_key(a, table, k0 + 16 * u + 4 * g, last_page);
+      if constexpr (kWide) {
+        pg.k[u] = ((const_i32_ptr)table)[min((k0 + 16 * u) >> a.page_shift, last_page)];
+      } else {
+        pg.k[u] = table[min((k0 + 16 * u + i) >> a.page_shift, last_page)];
+        pg.v[u] = table[min((k0 + 16 * u + 4 * g) >> a.page_shift, last_page)];
+      }
     }
     return pg;
   };
@@ -354,20 +370,21 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
   auto load_k = [&](int k0, const Pages& pg) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const char* row = row_of(a, pg.k[u], 2 * h, k0 + 16 * u + i);
+      const char* row = row_of(a, pg.k[u], 2 * h, k0 + 16 * u + (kWide ? 0 : i));
 #pragma unroll
-      for (int n = 0; n < NP; ++n) kr[u][n] = *reinterpret_cast<const u32x4_t*>(row + k_off[n]);
-      ks[u] = *scale_of(a, pg.v[u], 2 * h, k0 + 16 * u + 4 * g);
+      for (int n = 0; n < NP; ++n) kr[u][n] = *reinterpret_cast<const u32x4_t*>(row + here(k_off[n]));
+      ks[u] = kWide ? scale_of(a, pg.k[u], 2 * h, k0 + 16 * u)[here(sc_off)] : *scale_of(a, pg.v[u], 2 * h, k0 + 16 * u + 4 * g);
     }
   };
   auto load_v = [&](int k0, const Pages& pg) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const char* row = row_of(a, pg.v[u], 2 * h + 1, k0 + 16 * u + 4 * g) + v_off;
-      vs[u] = *scale_of(a, pg.v[u], 2 * h + 1, k0 + 16 * u + 4 * g);
+      const int page = kWide ? pg.k[u] : pg.v[u];
+      const char* row = row_of(a, page, 2 * h + 1, k0 + 16 * u + (kWide ? 0 : 4 * g));
+      vs[u] = kWide ? scale_of(a, page, 2 * h + 1, k0 + 16 * u)[here(sc_off)] : *scale_of(a, page, 2 * h + 1, k0 + 16 * u + 4 * g);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(row + r * dim);
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(row + here(v_off[r]));
         if constexpr (NV == 1) {
           vr[u][r][0] = src[0];
         } else if constexpr (NV == 2) {
@@ -384,13 +401,13 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
 
   const float cap = a.p.logits_soft_cap, inv_cap = kCap ? 1.f / cap : 0.f;
   const float c_scale = kCap ? a.p.softmax_scale : a.p.softmax_scale * kLog2e, cap2 = cap * kLog2e;
-  Pages pg_next = {};
-  {
-    const Pages pg = load_pages(k_begin);
-    load_k(k_begin, pg);
-    load_v(k_begin, pg);
-    if (k_begin + stride < k_end) pg_next = load_pages(k_begin + stride);
-  }
+  // Loads run ahead without a branch, so that every path to a wait has the same loads behind it: the last tile reads itself
+  // again (from the caches).
+  Pages pg = load_pages(k_begin), pg_next = load_pages(k_begin + stride);
+  load_k(k_begin, pg);
+  in_order();
+  load_v(k_begin, pg);
+  in_order();
   for (int k0 = k_begin; k0 < k_end; k0 += stride) {
     f32x4_t sa[MT][2];
 #pragma unroll
@@ -410,12 +427,18 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
       }
     float c[2] = {ks[0] * c_scale, ks[1] * c_scale}, w[2] = {vs[0], vs[1]};
     const bool more = k0 + stride < k_end;
-    Pages pg_after = {};
-    if (more) {
-      if (k0 + 2 * stride < k_end) pg_after = load_pages(k0 + 2 * stride);
-      load_k(k0 + stride, pg_next);
+    const int ahead = more ? k0 + stride : k0;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      pg.k[u] = more ? pg_next.k[u] : pg.k[u];
+      pg.v[u] = more ? pg_next.v[u] : pg.v[u];
     }
+    pg_next = load_pages(k0 + 2 * stride);
+    in_order();
+    load_k(ahead, pg);
+    in_order();
     const bool edge = k0 < full_lo || k0 + 32 > full_hi;
+    const int window = a.p.sliding_window > 0 ? a.p.sliding_window : 0x40000000;  // hi - window: the row's first key, or below 0
     if (kCap || edge) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -425,7 +448,7 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float x = scaled<kCap>(sa[mt][u][r], c[u], cap2, inv_cap);
-            sa[mt][u][r] = !edge || (k + r >= lo[mt] && k + r < hi[mt]) ? x : -INFINITY;
+            sa[mt][u][r] = !edge || (k + r < hi[mt] && k + r >= hi[mt] - window) ? x : -INFINITY;
           }
         c[u] = 1.f;
         if (edge) {  // what no row sees may be anything
@@ -491,8 +514,9 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
           for (int sp = 0; sp < kParts; ++sp) st.acc[mt][4 * j + b] = mfma(v, pf[mt][sp], st.acc[mt][4 * j + b]);
       }
     }
-    if (more) load_v(k0 + stride, pg_next);
-    pg_next = pg_after;
+    in_order();
+    load_v(ahead, pg);
+    in_order();
   }
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) st.l[mt] = row_groups_sum(st.l[mt]);
@@ -506,11 +530,11 @@ struct ThinLds {
 
 // A run of keys [ka, kb) (from the range's first key rounded down to 32) of one (sequence, kv head) with R <= 16 rows.
 // `self`: this workgroup's place in the cut; x0: the item's first position in the stream.
-template <int kCode, int D, typename T, int kParts, bool kCap>
+template <int kCode, int D, typename T, int kParts, bool kCap, bool kWide>
 __device__ __forceinline__ void thin_item(Args& a, const Seq& q, int s, int h, int ka, int kb, const Cut& cut, int self, int64_t x0,
                                           ThinLds<D>& lds, int* lds_flag) {
   constexpr int NO = D / 16;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
   const int G = a.group, R = q.q_len * G, dim = a.p.head_dim;
   const Range range = key_range(a, q, 0, q.q_len);
   const int base = range.first & ~31, keys = range.end - base;
@@ -519,7 +543,6 @@ __device__ __forceinline__ void thin_item(Args& a, const Seq& q, int s, int h, i
   // keys of row i
   const int pos = q.kv_len - q.q_len + token;
   const int hi = real ? pos + 1 : 0;
-  const int lo = a.p.sliding_window > 0 ? max(static_cast<int>(max(static_cast<int64_t>(pos) - a.p.sliding_window + 1, static_cast<int64_t>(0))), 0) : 0;
   const int full_lo = a.p.sliding_window > 0 ? max(q.kv_len - a.p.sliding_window, 0) : 0;  // keys every row sees
   const int full_hi = q.kv_len - q.q_len + 1;
 
@@ -530,7 +553,7 @@ __device__ __forceinline__ void thin_item(Args& a, const Seq& q, int s, int h, i
     for (int k = 0; k < D / 32; ++k) load_q<T, kParts>(row, real, 16 * (g + 4 * (k >> 1)) + 8 * (k & 1), dim, qf[0][k]);
   }
   RowState<1, D> st;
-  walk<kCode, D, kParts, kCap, 1>(a, q, s, h, qf, {lo}, {hi}, range, full_lo, full_hi, base + ka + 32 * wave, base + ((min(kb, keys) + 31) & ~31), 128, st);
+  walk<kCode, D, kParts, kCap, kWide, 1>(a, q, s, h, qf, {hi}, range, full_lo, full_hi, base + ka + 32 * wave, base + ((min(kb, keys) + 31) & ~31), 128, st);
   const auto& acc = st.acc[0];
   const float m = st.m[0], l = st.l[0];
 
@@ -601,22 +624,12 @@ __device__ __forceinline__ void thin_item(Args& a, const Seq& q, int s, int h, i
   if (NO * (4 * g + wave) < dim) store_row<T, NO>(dst + NO * (4 * g + wave), o);
 }
 
-template <int D>
-struct TileLds {
-  bf16x8_t k[2][quant_step_keys<D>() / 16][D / 32][64];  // buffer, 16 keys, 32 elements, lane
-  bf16x8_t v[2][quant_step_keys<D>() / 32][D / 16][64];  // buffer, 32 keys, output tile, lane
-  float ks[2][quant_step_keys<D>() / 4];
-  float vs[2][quant_step_keys<D>() / 4];
-};
-
 // A run of keys [ka, kb) of one tile of rows.
-template <int kCode, int D, typename T, int kParts, bool kCap>
+template <int kCode, int D, typename T, int kParts, bool kCap, bool kWide>
 __device__ __forceinline__ void tile_item(Args& a, const Seq& q, int s, int hs, int tile, int ka, int kb, const Cut& cut, int self, int64_t x0,
-                                          TileLds<D>& lds, int* lds_flag) {
-  constexpr int kStep = quant_step_keys<D>(), kRowTiles = quant_row_tiles<D, kParts>();
-  constexpr int NP = D / 64, NO = D / 16, kSub = kStep / 16, kBlocks = kStep / 32;
-  constexpr int kUnitsK = kSub * NP / 4, kUnitsV = (kBlocks * NP + 3) / 4;  // per wavefront
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+                                          int* lds_flag) {
+  constexpr int kRowTiles = quant_row_tiles<D, kParts>(), NO = D / 16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
   const int dim = a.p.head_dim;
   const int h = hs / a.subs, sub = hs - h * a.subs;
   const int t0 = tile * a.tile_tokens, t1 = min(t0 + a.tile_tokens, q.q_len);
@@ -624,248 +637,36 @@ __device__ __forceinline__ void tile_item(Args& a, const Seq& q, int s, int hs, 
   const int base = range.first & ~31, keys = range.end - base;
   const int q_base = q.kv_len - q.q_len;
 
-  // row tile m of this wavefront, row i
-  int token[kRowTiles], head[kRowTiles], lo[kRowTiles], hi[kRowTiles];
+  // row i of row tile m of this wavefront: its token in the sequence (negative: none) and its head
+  struct Row {
+    int token, head;
+  };
+  auto row_of_tile = [&](int mt) {
+    const int rr = (wave * kRowTiles + mt) * 16 + i;
+    const int dt = rr / a.tile_group, gg = sub * a.tile_group + rr - dt * a.tile_group;
+    return Row{dt < t1 - t0 && gg < a.group ? t0 + dt : -1, h * a.group + gg};
+  };
+  int hi[kRowTiles];
   bf16x8_t qf[kRowTiles][D / 32][kParts];
 #pragma unroll
   for (int mt = 0; mt < kRowTiles; ++mt) {
-    const int rr = (wave * kRowTiles + mt) * 16 + i;
-    const int dt = rr / a.tile_group, gg = sub * a.tile_group + rr - dt * a.tile_group;
-    const bool real = dt < t1 - t0 && gg < a.group;
-    token[mt] = real ? t0 + dt : -1;
-    head[mt] = h * a.group + gg;
-    const int pos = q_base + t0 + dt;
-    hi[mt] = real ? pos + 1 : 0;
-    lo[mt] = a.p.sliding_window > 0 ? static_cast<int>(max(static_cast<int64_t>(pos) - a.p.sliding_window + 1, static_cast<int64_t>(0))) : 0;
-    const T* row = static_cast<const T*>(a.p.queries) + (q.q0 + (real ? token[mt] : 0)) * a.p.query_token_stride + (real ? head[mt] : 0) * a.p.query_head_stride;
+    const Row row = row_of_tile(mt);
+    const bool real = row.token >= 0;
+    hi[mt] = real ? q_base + row.token + 1 : 0;
+    const T* src = static_cast<const T*>(a.p.queries) + (q.q0 + (real ? row.token : 0)) * a.p.query_token_stride + (real ? row.head : 0) * a.p.query_head_stride;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) load_q<T, kParts>(row, real, 16 * (g + 4 * (k >> 1)) + 8 * (k & 1), dim, qf[mt][k]);
+    for (int k = 0; k < D / 32; ++k) load_q<T, kParts>(src, real, 16 * (g + 4 * (k >> 1)) + 8 * (k & 1), dim, qf[mt][k]);
   }
   const int full_lo = a.p.sliding_window > 0 ? max(q_base + t1 - a.p.sliding_window, 0) : 0;  // keys every row sees
   const int full_hi = q_base + t0 + 1;
-  f32x4_t acc[kRowTiles][NO];
-  float m[kRowTiles], l[kRowTiles];
-#pragma unroll
-  for (int mt = 0; mt < kRowTiles; ++mt) {
-    m[mt] = kNoKey, l[mt] = 0.f;
-#pragma unroll
-    for (int n = 0; n < NO; ++n) acc[mt][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  }
-
-  const int32_t* __restrict__ table = a.p.block_tables + static_cast<size_t>(s) * a.p.pages_per_seq;
-  const int last_page = max(q.kv_len - 1, 0) >> a.page_shift;
-  u32x4_t kr[kUnitsK];
-  uint32_t vr[kUnitsV][2][4];
-  float k_scale = 0.f, v_scale = 0.f;  // of four keys of the step, the first lanes of wavefront 0
-  // K unit x: 16 keys, 16 elements a lane; V unit x: 32 keys (8 a lane), 64 elements (4 a lane)
-  auto load_k = [&](int k0) {
-#pragma unroll
-    for (int n = 0; n < kUnitsK; ++n) {
-      const int x = wave * kUnitsK + n, u = x / NP, piece = g + 4 * (x % NP);
-      const int k = k0 + 16 * u + i;
-      kr[n] = *reinterpret_cast<const u32x4_t*>(row_of(a, page_of_key(a, table, k, last_page), 2 * h, k) + (16 * piece < dim ? 16 * piece : 0));
-    }
-    if (threadIdx.x < kStep / 4) {
-      const int k = k0 + 4 * threadIdx.x;
-      k_scale = *scale_of(a, page_of_key(a, table, k, last_page), 2 * h, k);
-    }
-  };
-  auto load_v = [&](int k0) {
-#pragma unroll
-    for (int n = 0; n < kUnitsV; ++n) {
-      const int x = (wave * kUnitsV + n) % (kBlocks * NP), b = x / NP, d = 64 * (x % NP) + 4 * i;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int k = k0 + 32 * b + 16 * u + 4 * g;
-        const char* row = row_of(a, page_of_key(a, table, k, last_page), 2 * h + 1, k) + (d < dim ? d : 0);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) vr[n][u][r] = *reinterpret_cast<const uint32_t*>(row + r * dim);
-      }
-    }
-    if (threadIdx.x < kStep / 4) {
-      const int k = k0 + 4 * threadIdx.x;
-      v_scale = *scale_of(a, page_of_key(a, table, k, last_page), 2 * h + 1, k);
-    }
-  };
-  const float cap = a.p.logits_soft_cap, inv_cap = kCap ? 1.f / cap : 0.f;
-  const float c_scale = kCap ? a.p.softmax_scale : a.p.softmax_scale * kLog2e, cap2 = cap * kLog2e;
-  auto in_range = [&](int k, int n) { return k + n > range.first && k < range.end; };  // any of n keys from k on
-  auto store_k = [&](int k0, int buf) {
-#pragma unroll
-    for (int n = 0; n < kUnitsK; ++n) {
-      const int x = wave * kUnitsK + n, u = x / NP, np = x % NP;
-      bf16x8_t op[2];
-      widen16<kCode>(kr[n], op);
-      lds.k[buf][u][2 * np][lane] = op[0];
-      lds.k[buf][u][2 * np + 1][lane] = op[1];
-    }
-    if (threadIdx.x < kStep / 4) lds.ks[buf][threadIdx.x] = in_range(k0 + 4 * threadIdx.x, 4) ? k_scale * c_scale : 0.f;
-  };
-  auto store_v = [&](int k0, int buf) {
-    const bool edge = k0 < range.first || k0 + kStep > range.end;
-#pragma unroll
-    for (int n = 0; n < kUnitsV; ++n) {
-      const int x = wave * kUnitsV + n, b = x / NP, j = x % NP;
-      if (x >= kBlocks * NP) break;
-      if (edge) {  // what no row of the tile sees may be anything
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) vr[n][u][r] = in_range(k0 + 32 * b + 16 * u + 4 * g + r, 1) ? vr[n][u][r] : 0u;
-      }
-      uint32_t pair[4][4];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        widen_pairs<kCode>(vr[n][u][0], vr[n][u][1], pair[2 * u]);
-        widen_pairs<kCode>(vr[n][u][2], vr[n][u][3], pair[2 * u + 1]);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        lds.v[buf][b][4 * j + e][lane] = __builtin_bit_cast(bf16x8_t, u32x4_t{pair[0][e], pair[1][e], pair[2][e], pair[3][e]});
-    }
-    if (threadIdx.x < kStep / 4) lds.vs[buf][threadIdx.x] = in_range(k0 + 4 * threadIdx.x, 4) ? v_scale : 0.f;
-  };
-  // The loop is a pipeline of two stages, so that the matrix unit always has work beside the vector unit's: while the
-  // probabilities of step t are taken, the logits of step t + 1 are multiplied; while the outputs of step t are
-  // multiplied, the codes of K of step t + 2 and of V of step t + 1 are widened into LDS.  One barrier a step: K (t + 2)
-  // replaces K (t), whose last reads lie before the barrier, and V (t + 1) replaces V (t - 1), likewise.
-  typedef f32x4_t Scores[kRowTiles][kSub];
-  auto multiply_k = [&](Scores& sa, int buf) {
-#pragma unroll
-    for (int u = 0; u < kSub; ++u) {
-#pragma unroll
-      for (int mt = 0; mt < kRowTiles; ++mt) sa[mt][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < D / 32; ++k) {
-        const bf16x8_t op = lds.k[buf][u][k][lane];
-#pragma unroll
-        for (int mt = 0; mt < kRowTiles; ++mt)
-#pragma unroll
-          for (int sp = 0; sp < kParts; ++sp) sa[mt][u] = mfma(op, qf[mt][k][sp], sa[mt][u]);
-      }
-    }
-  };
-  // Scales (not negative), cap and mask of a step's logits, and the running maximum's move.  c: what is left to multiply by.
-  auto prepare = [&](Scores& sa, float (&c)[kSub], int k0, int buf) {
-#pragma unroll
-    for (int u = 0; u < kSub; ++u) c[u] = lds.ks[buf][4 * u + g];
-    const bool edge = k0 < full_lo || k0 + kStep > full_hi;
-    if (kCap || edge) {
-#pragma unroll
-      for (int u = 0; u < kSub; ++u) {
-#pragma unroll
-        for (int mt = 0; mt < kRowTiles; ++mt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int k = k0 + 16 * u + 4 * g + r;
-            const float x = scaled<kCap>(sa[mt][u][r], c[u], cap2, inv_cap);
-            sa[mt][u][r] = !edge || (k >= lo[mt] && k < hi[mt]) ? x : -INFINITY;
-          }
-        c[u] = 1.f;
-      }
-    }
-    float top[kRowTiles];
-    bool up = false;
-#pragma unroll
-    for (int mt = 0; mt < kRowTiles; ++mt) {
-#pragma unroll
-      for (int u = 0; u < kSub; ++u) {
-        const float x = fmaxf(fmaxf(fmaxf(sa[mt][u][0], sa[mt][u][1]), sa[mt][u][2]), sa[mt][u][3]) * c[u];
-        top[mt] = u == 0 ? x : fmaxf(top[mt], x);
-      }
-      up |= top[mt] > m[mt] + kLazy;
-    }
-    if (__any(up)) {
-#pragma unroll
-      for (int mt = 0; mt < kRowTiles; ++mt) {
-        const float m_new = fmaxf(m[mt], row_groups_max(top[mt]));
-        const float alpha = __builtin_amdgcn_exp2f(m[mt] - m_new);
-#pragma unroll
-        for (int n = 0; n < NO; ++n) acc[mt][n] *= alpha;
-        l[mt] *= alpha;
-        m[mt] = m_new;
-      }
-    }
-  };
-  auto probabilities = [&](const Scores& sa, const float (&c)[kSub], int buf, bf16x8_t (&pf)[kBlocks][kRowTiles][kParts]) {
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-      for (int mt = 0; mt < kRowTiles; ++mt) {
-        float pv[8];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float w = lds.vs[buf][8 * b + 4 * u + g];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(sa[mt][2 * b + u][r], c[2 * b + u], -m[mt]));
-            l[mt] += p;
-            pv[4 * u + r] = p * w;
-          }
-        }
-        split<kParts>(pv, pf[b][mt]);
-      }
-  };
-
-  const int t_begin = ka / kStep, t_end = (min(kb, keys) + kStep - 1) / kStep;
-  auto key_of = [&](int t) { return base + t * kStep; };
-  __syncthreads();  // LDS may hold what came before
-  if (t_begin < t_end) {
-    Scores sa;
-    float c[kSub];
-    load_k(key_of(t_begin));
-    load_v(key_of(t_begin));
-    store_k(key_of(t_begin), 0);
-    if (t_begin + 1 < t_end) load_k(key_of(t_begin + 1));
-    store_v(key_of(t_begin), 0);
-    if (t_begin + 1 < t_end) {
-      load_v(key_of(t_begin + 1));
-      store_k(key_of(t_begin + 1), 1);
-      if (t_begin + 2 < t_end) load_k(key_of(t_begin + 2));
-    }
-    __syncthreads();
-    multiply_k(sa, 0);
-    prepare(sa, c, key_of(t_begin), 0);
-    for (int t = t_begin; t < t_end; ++t) {
-      const int buf = (t - t_begin) & 1;
-      if (t > t_begin) __syncthreads();
-      const bool more = t + 1 < t_end;
-      Scores sb;
-      bf16x8_t pf[kBlocks][kRowTiles][kParts];
-      if (more) multiply_k(sb, buf ^ 1);
-      probabilities(sa, c, buf, pf);
-      if (more) {
-        if (t + 2 < t_end) {
-          store_k(key_of(t + 2), buf);
-          if (t + 3 < t_end) load_k(key_of(t + 3));
-        }
-        store_v(key_of(t + 1), buf ^ 1);
-        if (t + 2 < t_end) load_v(key_of(t + 2));
-      }
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-        for (int n = 0; n < NO; ++n) {
-          const bf16x8_t v = lds.v[buf][b][n][lane];
-#pragma unroll
-          for (int mt = 0; mt < kRowTiles; ++mt)
-#pragma unroll
-            for (int sp = 0; sp < kParts; ++sp) acc[mt][n] = mfma(v, pf[b][mt][sp], acc[mt][n]);
-        }
-      if (more) {
-        prepare(sb, c, key_of(t + 1), buf ^ 1);
-#pragma unroll
-        for (int mt = 0; mt < kRowTiles; ++mt)
-#pragma unroll
-          for (int u = 0; u < kSub; ++u) sa[mt][u] = sb[mt][u];
-      }
-    }
-  }
-#pragma unroll
-  for (int mt = 0; mt < kRowTiles; ++mt) l[mt] = row_groups_sum(l[mt]);
+  RowState<kRowTiles, D> st;
+  walk<kCode, D, kParts, kCap, kWide, kRowTiles>(a, q, s, h, qf, hi, range, full_lo, full_hi, base + ka, base + ((min(kb, keys) + 31) & ~31), 32, st);
+  auto& acc = st.acc;
+  auto& m = st.m;
+  auto& l = st.l;
 
   if (ka > 0 || kb < keys) {
-    const Parts parts = parts_of(cut, x0, range.end - range.first, kStep);
+    const Parts parts = parts_of(cut, x0, range.end - range.first, kTileStep);
     const int slots = 2 * a.grid;
     const auto o_rsrc = rsrc_of(a.tile_o, static_cast<uint64_t>(slots) * 64 * kRowTiles * D * 4);
     const int part = self - parts.first;
@@ -902,19 +703,18 @@ __device__ __forceinline__ void tile_item(Args& a, const Seq& q, int s, int hs, 
   }
 #pragma unroll
   for (int mt = 0; mt < kRowTiles; ++mt) {
-    if (token[mt] < 0) continue;
+    const Row row = row_of_tile(mt);
+    if (row.token < 0) continue;
     float weight;
-    add_sinks(a, head[mt], m[mt], l[mt], weight);
+    add_sinks(a, row.head, m[mt], l[mt], weight);
     const float f = l[mt] > 0.f ? weight / l[mt] : 0.f;
-    T* dst = static_cast<T*>(a.p.out) + (static_cast<size_t>(q.q0 + token[mt]) * a.p.num_q_heads + head[mt]) * dim;
+    T* dst = static_cast<T*>(a.p.out) + (static_cast<size_t>(q.q0 + row.token) * a.p.num_q_heads + row.head) * dim;
 #pragma unroll
-    for (int j = 0; j < NP; ++j) {
-      float o[16];
+    for (int r = 0; r < 4; ++r) {
+      float o[NO];
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[4 * r + e] = acc[mt][4 * j + e][r] * f;
-      if (64 * j + 16 * g < dim) store_row<T, 16>(dst + 64 * j + 16 * g, o);
+      for (int n = 0; n < NO; ++n) o[n] = acc[mt][n][r] * f;
+      if (NO * (4 * g + r) < dim) store_row<T, NO>(dst + NO * (4 * g + r), o);
     }
   }
 }
@@ -942,7 +742,6 @@ template <int D>
 struct Lds {
   union {
     ThinLds<D> thin;
-    TileLds<D> tile;
   };
   SchedLds sched;
 };
@@ -962,7 +761,7 @@ __device__ __forceinline__ Run uniform(const Run& r) {
 }
 
 // The two streams are functions of their own, so that the registers of one loop are not shared out by the other's.
-template <int kCode, int D, typename T, int kParts, bool kCap>
+template <int kCode, int D, typename T, int kParts, bool kCap, bool kWide>
 __device__ __attribute__((noinline)) void thin_phase(uint64_t args) {
   Args& a = *reinterpret_cast<Args*>(uniform(static_cast<int64_t>(args)));
   Lds<D>& lds = lds_of<D>();
@@ -982,7 +781,7 @@ __device__ __attribute__((noinline)) void thin_phase(uint64_t args) {
       const int end = static_cast<int>(min(static_cast<int64_t>(len), begin + (run.x_end - x)));
       const int ka = begin >= keys ? all : begin / kThinStep * kThinStep, kb = end >= keys ? all : end / kThinStep * kThinStep;
       if (ka < kb || (keys == 0 && begin == 0))
-        thin_item<kCode, D, T, kParts, kCap>(a, q, s, h, keys == 0 ? 0 : ka, kb, run.cut, run.self, x - begin, lds.thin, &lds.sched.flag);
+        thin_item<kCode, D, T, kParts, kCap, kWide>(a, q, s, h, keys == 0 ? 0 : ka, kb, run.cut, run.self, x - begin, lds.thin, &lds.sched.flag);
       x += end - begin;
     }
     off = 0;
@@ -990,9 +789,9 @@ __device__ __attribute__((noinline)) void thin_phase(uint64_t args) {
   }
 }
 
-template <int kCode, int D, typename T, int kParts, bool kCap>
+template <int kCode, int D, typename T, int kParts, bool kCap, bool kWide>
 __device__ __attribute__((noinline)) void tile_phase(uint64_t args) {
-  constexpr int kStep = quant_step_keys<D>();
+  constexpr int kStep = kTileStep;
   Args& a = *reinterpret_cast<Args*>(uniform(static_cast<int64_t>(args)));
   Lds<D>& lds = lds_of<D>();
   const Run run = uniform(lds.sched.run[1]);
@@ -1021,7 +820,7 @@ __device__ __attribute__((noinline)) void tile_phase(uint64_t args) {
         const int end = static_cast<int>(min(static_cast<int64_t>(item), begin + (run.x_end - x)));
         const int ka = begin >= keys ? all : begin / kStep * kStep, kb = end >= keys ? all : end / kStep * kStep;
         if (ka < kb || (keys == 0 && begin == 0))
-          tile_item<kCode, D, T, kParts, kCap>(a, q, s, h, tile, keys == 0 ? 0 : ka, kb, run.cut, run.self, x - begin, lds.tile, &lds.sched.flag);
+          tile_item<kCode, D, T, kParts, kCap, kWide>(a, q, s, h, tile, keys == 0 ? 0 : ka, kb, run.cut, run.self, x - begin, &lds.sched.flag);
         x += end - begin;
       }
     }
@@ -1030,7 +829,7 @@ __device__ __attribute__((noinline)) void tile_phase(uint64_t args) {
   }
 }
 
-template <int kCode, int D, typename T, int kParts, bool kCap>
+template <int kCode, int D, typename T, int kParts, bool kCap, bool kWide>
 __global__ __launch_bounds__(256, 2) void quant_attention_kernel(QuantArgs) {
   Args& a = *(Args*)__builtin_amdgcn_kernarg_segment_ptr();
   SchedLds& sched = lds_of<D>().sched;
@@ -1100,8 +899,8 @@ __global__ __launch_bounds__(256, 2) void quant_attention_kernel(QuantArgs) {
   for (int k = 0; k < 2; ++k) {
     const int c = (k == 0) == thin_first ? 0 : 1;
     const uint64_t args = reinterpret_cast<uint64_t>(&a);
-    if (c == 0 && has[0]) thin_phase<kCode, D, T, kParts, kCap>(args);
-    if (c == 1 && has[1]) tile_phase<kCode, D, T, kParts, kCap>(args);
+    if (c == 0 && has[0]) thin_phase<kCode, D, T, kParts, kCap, kWide>(args);
+    if (c == 1 && has[1]) tile_phase<kCode, D, T, kParts, kCap, kWide>(args);
   }
 
   // Rows in front of the first sequence and behind the last are zeros.
@@ -1126,8 +925,12 @@ int launch_quant_codes(const QuantArgs& a, hipStream_t stream) {
   };
   auto width = [&](auto d) {
     constexpr int D = decltype(d)::value;
-    if (f32) return cap ? go(quant::quant_attention_kernel<kCode, D, float, 3, true>) : go(quant::quant_attention_kernel<kCode, D, float, 3, false>);
-    return cap ? go(quant::quant_attention_kernel<kCode, D, bf16_t, 1, true>) : go(quant::quant_attention_kernel<kCode, D, bf16_t, 1, false>);
+    auto pages = [&](auto wide) {
+      constexpr bool W = decltype(wide)::value;
+      if (f32) return cap ? go(quant::quant_attention_kernel<kCode, D, float, 3, true, W>) : go(quant::quant_attention_kernel<kCode, D, float, 3, false, W>);
+      return cap ? go(quant::quant_attention_kernel<kCode, D, bf16_t, 1, true, W>) : go(quant::quant_attention_kernel<kCode, D, bf16_t, 1, false, W>);
+    };
+    return a.page_shift >= 4 ? pages(std::true_type{}) : pages(std::false_type{});
   };
   if (a.p.head_dim <= 64) return width(std::integral_constant<int, 64>{});
   if (a.p.head_dim <= 128) return width(std::integral_constant<int, 128>{});

@@ -8,10 +8,14 @@ namespace rpa {
 namespace {
 
 int padded_dim(const RpaQuantParams& p) { return p.head_dim <= 64 ? 64 : p.head_dim <= 128 ? 128 : 256; }
+// Rows of a tile of the second stream: what the instantiation that launch_quant_codes picks has.
 int tile_rows(const RpaQuantParams& p) {
   const bool f32 = p.dtype == RPA_DTYPE_F32;
-  if (padded_dim(p) == 256) return 64 * (f32 ? quant_row_tiles<256, 3>() : quant_row_tiles<256, 1>());
-  return 64 * (f32 ? quant_row_tiles<128, 3>() : quant_row_tiles<128, 1>());
+  switch (padded_dim(p)) {
+    case 64: return 64 * (f32 ? quant_row_tiles<64, 3>() : quant_row_tiles<64, 1>());
+    case 128: return 64 * (f32 ? quant_row_tiles<128, 3>() : quant_row_tiles<128, 1>());
+    default: return 64 * (f32 ? quant_row_tiles<256, 3>() : quant_row_tiles<256, 1>());
+  }
 }
 int grid_of() { return std::max(8, 2 * device_cu_count() / 8 * 8); }  // two workgroups per compute unit, the same number on each XCD
 

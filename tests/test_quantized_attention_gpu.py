@@ -52,7 +52,7 @@ def test_splits(seqs, kind):
     run(Batch(seqs, q_heads=8, kv_heads=2, dim=128, page=16, block=16, kind=kind, seed=len(seqs)))
 
 
-@pytest.mark.parametrize("group", [1, 2, 3, 7, 16, 17, 40])
+@pytest.mark.parametrize("group", [1, 2, 3, 7, 16, 17, 40, 65, 130, 200])
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_group_sizes(group, dtype):
     run(Batch([(1, 200), (3, 77), (6, 6), (40, 90), (1, 1)], q_heads=2 * group, kv_heads=2, dim=64, page=16, block=4, kind="e4m3", dtype=dtype, seed=group))

@@ -167,7 +167,7 @@ def test_c_attention_arguments():
     lib = _native.load()
     size = lib.rpa_quant_workspace_bytes(ctypes.byref(filled("RpaQuantParams")))
     assert size >= 256 and lib.rpa_quant_workspace_bytes(None) == 0
-    for field, value, rc in (("num_q_heads", 3, -1), ("max_num_seqs", 0, -1), ("pages_per_seq", 0, -1), ("sliding_window", -1, -1), ("softmax_scale", float("nan"), -1),
+    for field, value, rc in (("num_q_heads", 3, -1), ("max_num_seqs", 0, -1), ("pages_per_seq", 0, -1), ("pages_per_seq", (1 << 26) + 1, -2), ("sliding_window", -1, -1), ("softmax_scale", float("nan"), -1),
                              ("logits_soft_cap", float("inf"), -1), ("flags", 1, -1), ("num_sinks", -1, -1), ("query_token_stride", 100, -1),
                              ("query_head_stride", -64, -1), ("queries", 0x1004, -1), ("out", None, -1), ("workspace", None, -3), ("workspace_bytes", size - 1, -3),
                              ("workspace", 0x1010, -3)):
