@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 # RPA_LIBRARY points at another build of the same library (e.g. one compiled with different tile constants).
@@ -319,16 +320,46 @@ def load() -> ctypes.CDLL:
     lib.rpa_ragged_decode_launch.argtypes = [ctypes.POINTER(RpaRaggedDecodeParams), ctypes.c_void_p]
     lib.rpa_quant_workspace_bytes.restype = ctypes.c_uint64
     lib.rpa_quant_workspace_bytes.argtypes = [ctypes.POINTER(RpaQuantParams)]
-    for name, struct in (("rpa_quant_fwd_launch", RpaQuantParams), ("rpa_quant_update_launch", RpaQuantUpdateParams),
+    for name, params in (("rpa_quant_fwd_launch", RpaQuantParams), ("rpa_quant_update_launch", RpaQuantUpdateParams),
                          ("rpa_quant_gather_launch", RpaQuantGatherParams), ("rpa_block_tables_launch", RpaBlockTablesParams)):
         getattr(lib, name).restype = ctypes.c_int
-        getattr(lib, name).argtypes = [ctypes.POINTER(struct), ctypes.c_void_p]
+        getattr(lib, name).argtypes = [ctypes.POINTER(params), ctypes.c_void_p]
     if lib.rpa_abi_version() != RPA_ABI_VERSION:
         raise NativeLibraryError(
             f"{LIB_PATH} has ABI version {lib.rpa_abi_version()}, this package expects {RPA_ABI_VERSION}: rebuild it"
         )
     _lib = lib
     return lib
+
+
+_FORMATS = {ctypes.c_void_p: "Q", ctypes.c_uint64: "Q", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_uint32: "I", ctypes.c_float: "f"}
+
+
+class Entry:
+    """A C entry point of the shape ``int entry(const Params*, hipStream_t)``, called with the fields' values in order.
+
+    The values are packed at once into the bytes of the struct, a fifth of what setting its fields one by one costs
+    (pointers are integers here, 0 for null); a value outside its field's range is a ``ValueError``.
+    """
+
+    def __init__(self, name: str, params: type[ctypes.Structure]):
+        self.name = name
+        self.layout = struct.Struct("=" + "".join(_FORMATS[kind] for _, kind in params._fields_))
+        assert self.layout.size == ctypes.sizeof(params), f"{params.__name__} has padding"
+        self._function = None
+
+    def __call__(self, stream: int, *values) -> None:
+        fn = self._function
+        if fn is None:
+            fn = self._function = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, ctypes.c_void_p)(ctypes.cast(getattr(load(), self.name), ctypes.c_void_p).value)
+        try:
+            packed = self.layout.pack(*values)
+        except (struct.error, OverflowError) as e:
+            raise ValueError(f"{self.name}: an argument is out of range: {e}") from None
+        rc = fn(packed, stream)
+        if rc != 0:
+            kind = ValueError if rc in (-1, -2) else RuntimeError
+            raise kind(f"{self.name} refused the call ({rc}): {last_error()}")
 
 
 def last_error() -> str:

@@ -24,6 +24,8 @@ int check_pool(const P& p) {
     return fail(RPA_ERR_UNSUPPORTED, "scale_block=%d must be a power of two from 4 to page_size=%d", p.scale_block, p.page_size);
   if (static_cast<int64_t>(p.num_pages) * p.page_size > 0x7fffffff)
     return fail(RPA_ERR_UNSUPPORTED, "num_pages * page_size = %lld must be below 2^31", static_cast<long long>(p.num_pages) * p.page_size);
+  if (2 * static_cast<int64_t>(p.num_kv_heads) * p.page_size * p.head_dim > 0x7fffffff)
+    return fail(RPA_ERR_UNSUPPORTED, "a page of %lld bytes: it must be smaller than 2^31", 2 * static_cast<long long>(p.num_kv_heads) * p.page_size * p.head_dim);
   if (p.dtype != RPA_DTYPE_BF16 && p.dtype != RPA_DTYPE_F32)
     return fail(RPA_ERR_INVALID_ARGUMENT, "dtype=%d must be RPA_DTYPE_BF16 or RPA_DTYPE_F32", p.dtype);
   if (p.cache_dtype != RPA_DTYPE_INT8 && p.cache_dtype != RPA_DTYPE_FP8_E4M3 && p.cache_dtype != RPA_DTYPE_FP8_E5M2)

@@ -32,8 +32,8 @@ struct QuantArgs {
   int tile_group;   // rows of one token in a tile of the second stream: min(group, rows of a tile)
   int tile_tokens;  // tokens of a tile
   int subs;         // tiles side by side for the heads of one token, where they are more than a tile's rows
-  int grid;         // workgroups, a multiple of 8
-  uint32_t* tickets;        // [2 * grid], zero between launches
+  int grid;         // workgroups, a multiple of 16
+  uint32_t* tickets;        // [5 * grid], zero between launches: one for each workgroup's cut item of the first stream, four of the second
   float* thin_o;            // [2 * grid][16 * D] states of cut items of the first stream, as they lie in registers
   float* thin_ml;           // [2 * grid][16][2]
   float* tile_o;            // [2 * grid][rows * D]
@@ -49,6 +49,7 @@ constexpr int kThinStep = 128;     // keys a workgroup takes at once in the firs
 constexpr int kThinPad = 128;      // what an item of the first stream costs beyond its keys, in keys
 constexpr int kTilePad = 64;       // the same of the second
 constexpr int kThinLeast = 256;    // least run of keys per workgroup
+constexpr int kThinWhole = 2048;   // few items of up to so many keys are not cut
 constexpr int kTileLeast = 512;
 constexpr float kNoKey = -3.0e38f; // row maximum before any key
 constexpr float kLazy = 8.f;       // the running maximum follows when a logit passes it by 2^8
@@ -100,23 +101,47 @@ __device__ __forceinline__ int thin_keys(Args& a, const Seq& q) {
   return r.end - r.first;
 }
 
+// Lengths of sequence s, clipped to what the buffers hold; empty from sequence n on.  The loads do not wait for n.
 __device__ __forceinline__ Seq load_seq(Args& a, int n, int s) {
-  Seq q = {0, 0, 0};
-  if (s < n) {
-    q.q0 = min(max(a.p.query_start_loc[s], 0), a.p.total_tokens);
-    q.q_len = max(min(max(a.p.query_start_loc[s + 1], 0), a.p.total_tokens) - q.q0, 0);
-    const int64_t room = static_cast<int64_t>(a.p.pages_per_seq) << a.page_shift;
-    q.kv_len = static_cast<int>(min(static_cast<int64_t>(max(a.p.context_lens[s], 0)), room));
-  }
+  const int at = min(s, a.p.max_num_seqs - 1);
+  const int q0 = a.p.query_start_loc[at], q1 = a.p.query_start_loc[at + 1], len = a.p.context_lens[at];
+  Seq q;
+  q.q0 = min(max(q0, 0), a.p.total_tokens);
+  q.q_len = s < n ? max(min(max(q1, 0), a.p.total_tokens) - q.q0, 0) : 0;
+  q.kv_len = min(max(len, 0), a.p.pages_per_seq << a.page_shift);  // at most 2^30
   return q;
 }
 
-// A cut of a stream of `total` positions over `n` workgroups: run w is [bound(w), bound(w + 1)).
+// A cut of a stream of `total` positions over `n` workgroups: run w is [bound(w), bound(w + 1)).  Where the whole grid takes
+// part, two workgroups share a compute unit, and the one that was there first gets the larger part of its issue slots and
+// of its memory requests: with equal runs it ends at three quarters of the other's time.  So it gets the longer run: kFirstThin or
+// kFirstTile of kPairUnits, the other the rest.  The workgroups of an XCD hold `block` neighbouring runs, those of the first
+// workgroups in front or, where `back` is set, behind.
+constexpr int kPairUnits = 128, kFirstThin = 76, kFirstTile = 78;
+// 64-bit division where it is needed, 32-bit where that does.
+__device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
+  if (static_cast<uint64_t>(x | y) >> 32 == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
+  return x / y;
+}
 struct Cut {
-  int64_t total;
-  int n;
-  __device__ __forceinline__ int64_t bound(int w) const { return total * w / n; }
-  __device__ __forceinline__ int owner(int64_t x) const { return static_cast<int>(((x + 1) * n - 1) / total); }
+  int64_t per_unit, rest;  // positions of a unit; the first `rest` units have one more
+  int n, block, pair, lead;  // workgroups; a block of them; units of two runs, one of each half of a block; of the one in front
+  __device__ __forceinline__ void set(int64_t total) {
+    const int64_t units = static_cast<int64_t>(n) * pair / 2;
+    per_unit = divide(total, units);
+    rest = total - per_unit * units;
+  }
+  __device__ __forceinline__ int64_t bound(int w) const {
+    const int b = w / block, r = w - b * block, half = block / 2;
+    const int64_t u = static_cast<int64_t>(b) * half * pair + (r <= half ? r * lead : half * lead + (r - half) * (pair - lead));
+    return u * per_unit + min(u, rest);
+  }
+  __device__ __forceinline__ int owner(int64_t x) const {  // the run that holds position x
+    const int64_t big = rest * (per_unit + 1);
+    const int64_t u = x < big ? divide(x, per_unit + 1) : rest + divide(x - big, per_unit);
+    const int half = block / 2, b = static_cast<int>(divide(u, half * pair)), r = static_cast<int>(u - static_cast<int64_t>(b) * half * pair);
+    return b * block + (r < half * lead ? r / lead : half + (r - half * lead) / (pair - lead));
+  }
 };
 
 // Lengths of 64 sequences at a time, a lane each.
@@ -143,18 +168,6 @@ struct Window {
     return n;
   }
 };
-
-// Row of key k of a combined head, and its block's scale, in the page that the block table names (clamped here, where it is
-// used, so that nothing waits for it where it is loaded).
-__device__ __forceinline__ const char* row_of(Args& a, int page, int head, int k) {
-  const uint64_t line = static_cast<uint64_t>(clamp_page(page, a.p.num_pages)) * (2 * a.p.num_kv_heads) + head;
-  const uint64_t row = (line << a.page_shift) + (k & ((1 << a.page_shift) - 1));
-  return static_cast<const char*>(a.p.kv_cache) + row * a.p.head_dim;
-}
-__device__ __forceinline__ const float* scale_of(Args& a, int page, int head, int k) {
-  const uint64_t line = static_cast<uint64_t>(clamp_page(page, a.p.num_pages)) * (2 * a.p.num_kv_heads) + head;
-  return a.p.kv_scales + (line << (a.page_shift - a.block_shift)) + ((k & ((1 << a.page_shift) - 1)) >> a.block_shift);
-}
 
 // bf16 parts of eight fp32 values: part 0 is the value rounded, part 1 the rest of it rounded, part 2 the rest of that.
 template <int kParts>
@@ -347,10 +360,17 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
   const uint32_t sc_off = 4 * g >> a.block_shift;
 
   // Pages of 16 tokens and more (kWide): 16 keys have one page, whose address is scalar.  Shorter ones: a page for each
-  // lane's key of K and for each lane's four keys of V.
+  // lane's key of K and for each lane's four keys of V.  A page is fewer than 2^32 bytes.
   struct Pages {
     int k[2] = {0, 0}, v[2] = {0, 0};
   };
+  const int page_mask = (1 << a.page_shift) - 1;
+  const uint32_t head_bytes = static_cast<uint32_t>(dim) << a.page_shift, page_bytes = 2 * a.p.num_kv_heads * head_bytes;
+  const uint32_t head_scales = 1u << (a.page_shift - a.block_shift), page_scales = 2 * a.p.num_kv_heads * head_scales;
+  const char* k_codes = static_cast<const char*>(a.p.kv_cache) + static_cast<uint64_t>(2 * h) * head_bytes;
+  const float* k_scales = a.p.kv_scales + static_cast<uint64_t>(2 * h) * head_scales;
+  auto codes_at = [&](int page, int k) { return k_codes + (static_cast<uint64_t>(static_cast<uint32_t>(page)) * page_bytes + static_cast<uint32_t>((k & page_mask) * dim)); };
+  auto scales_at = [&](int page, int k) { return k_scales + (static_cast<uint64_t>(static_cast<uint32_t>(page)) * page_scales + static_cast<uint32_t>((k & page_mask) >> a.block_shift)); };
   auto load_pages = [&](int k0) {
     Pages pg;
 #pragma unroll
@@ -367,24 +387,29 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
   u32x4_t kr[2][NP];
   uint32_t vr[2][4][NV];
   float ks[2], vs[2];
+  const char* v_rows[2];    // where V of the tile in flight begins, and its scales: known when its K was asked for
+  const float* v_scale[2];
   auto load_k = [&](int k0, const Pages& pg) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const char* row = row_of(a, pg.k[u], 2 * h, k0 + 16 * u + (kWide ? 0 : i));
+      // the pages are clamped here, where they are used, so that nothing waits for them where they are loaded
+      const int page = clamp_page(pg.k[u], a.p.num_pages), v_page = kWide ? page : clamp_page(pg.v[u], a.p.num_pages);
+      const char* row = codes_at(page, k0 + 16 * u + (kWide ? 0 : i));
+      const float* sc = scales_at(v_page, k0 + 16 * u + (kWide ? 0 : 4 * g));
+      v_rows[u] = (kWide ? row : codes_at(v_page, k0 + 16 * u + 4 * g)) + head_bytes;
+      v_scale[u] = sc + head_scales;
 #pragma unroll
       for (int n = 0; n < NP; ++n) kr[u][n] = *reinterpret_cast<const u32x4_t*>(row + here(k_off[n]));
-      ks[u] = kWide ? scale_of(a, pg.k[u], 2 * h, k0 + 16 * u)[here(sc_off)] : *scale_of(a, pg.v[u], 2 * h, k0 + 16 * u + 4 * g);
+      ks[u] = kWide ? sc[here(sc_off)] : *sc;
     }
   };
-  auto load_v = [&](int k0, const Pages& pg) {
+  auto load_v = [&] {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int page = kWide ? pg.k[u] : pg.v[u];
-      const char* row = row_of(a, page, 2 * h + 1, k0 + 16 * u + (kWide ? 0 : 4 * g));
-      vs[u] = kWide ? scale_of(a, page, 2 * h + 1, k0 + 16 * u)[here(sc_off)] : *scale_of(a, page, 2 * h + 1, k0 + 16 * u + 4 * g);
+      vs[u] = kWide ? v_scale[u][here(sc_off)] : *v_scale[u];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(row + here(v_off[r]));
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(v_rows[u] + here(v_off[r]));
         if constexpr (NV == 1) {
           vr[u][r][0] = src[0];
         } else if constexpr (NV == 2) {
@@ -406,7 +431,7 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
   Pages pg = load_pages(k_begin), pg_next = load_pages(k_begin + stride);
   load_k(k_begin, pg);
   in_order();
-  load_v(k_begin, pg);
+  load_v();
   in_order();
   for (int k0 = k_begin; k0 < k_end; k0 += stride) {
     f32x4_t sa[MT][2];
@@ -515,7 +540,7 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
       }
     }
     in_order();
-    load_v(ahead, pg);
+    load_v();
     in_order();
   }
 #pragma unroll
@@ -600,17 +625,30 @@ __device__ __forceinline__ void thin_item(Args& a, const Seq& q, int s, int h, i
     top = kNoKey, sum = 0.f;
 #pragma unroll
     for (int n = 0; n < NO; ++n) o[n] = 0.f;
-    for (int k = 0; k < parts.count; ++k) {
-      const uint64_t both = __hip_atomic_load(reinterpret_cast<uint64_t*>(a.thin_ml) + slot_of(parts, k) * 16 + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const float mk = __uint_as_float(static_cast<uint32_t>(both)), lk = __uint_as_float(static_cast<uint32_t>(both >> 32));
-      const float t_new = fmaxf(top, mk), f = __builtin_amdgcn_exp2f(top - t_new), fk = __builtin_amdgcn_exp2f(mk - t_new);
-      top = t_new;
-      sum = sum * f + lk * fk;
+    constexpr int kAtOnce = 4;  // parts whose loads are in flight together
+    for (int k0 = 0; k0 < parts.count; k0 += kAtOnce) {
+      uint64_t both[kAtOnce];
+      u32x4_t y[kAtOnce][NO / 4];
 #pragma unroll
-      for (int n = 0; n < NO / 4; ++n) {
-        const f32x4_t y = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(o_rsrc, place(k, n), 0, kAgentScope));
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int k = min(k0 + j, parts.count - 1);
+        both[j] = __hip_atomic_load(reinterpret_cast<uint64_t*>(a.thin_ml) + slot_of(parts, k) * 16 + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[4 * n + e] = o[4 * n + e] * f + y[e] * fk;
+        for (int n = 0; n < NO / 4; ++n) y[j][n] = __builtin_amdgcn_raw_buffer_load_b128(o_rsrc, place(k, n), 0, kAgentScope);
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        if (k0 + j >= parts.count) break;
+        const float mk = __uint_as_float(static_cast<uint32_t>(both[j])), lk = __uint_as_float(static_cast<uint32_t>(both[j] >> 32));
+        const float t_new = fmaxf(top, mk), f = __builtin_amdgcn_exp2f(top - t_new), fk = __builtin_amdgcn_exp2f(mk - t_new);
+        top = t_new;
+        sum = sum * f + lk * fk;
+#pragma unroll
+        for (int n = 0; n < NO / 4; ++n) {
+          const f32x4_t z = __builtin_bit_cast(f32x4_t, y[j][n]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[4 * n + e] = o[4 * n + e] * f + z[e] * fk;
+        }
       }
     }
   }
@@ -626,8 +664,7 @@ __device__ __forceinline__ void thin_item(Args& a, const Seq& q, int s, int h, i
 
 // A run of keys [ka, kb) of one tile of rows.
 template <int kCode, int D, typename T, int kParts, bool kCap, bool kWide>
-__device__ __forceinline__ void tile_item(Args& a, const Seq& q, int s, int hs, int tile, int ka, int kb, const Cut& cut, int self, int64_t x0,
-                                          int* lds_flag) {
+__device__ __forceinline__ void tile_item(Args& a, const Seq& q, int s, int hs, int tile, int ka, int kb, const Cut& cut, int self, int64_t x0) {
   constexpr int kRowTiles = quant_row_tiles<D, kParts>(), NO = D / 16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
   const int dim = a.p.head_dim;
@@ -681,23 +718,36 @@ __device__ __forceinline__ void tile_item(Args& a, const Seq& q, int s, int hs, 
         __hip_atomic_store(ml_at(part, mt), both, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     }
-    if (!last_part(a.tickets + a.grid + parts.first, parts.count, lds_flag)) return;
+    // A wavefront's rows are its own: it draws a ticket for them, and the wavefront that draws the last one adds them up.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    uint32_t* ticket = a.tickets + a.grid + 4 * parts.first + wave;
+    uint32_t drawn = 0;
+    if (lane == 0) drawn = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (__builtin_amdgcn_readfirstlane(drawn) + 1 != static_cast<uint32_t>(parts.count)) return;
+    if (lane == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
     for (int mt = 0; mt < kRowTiles; ++mt) {
       m[mt] = kNoKey, l[mt] = 0.f;
 #pragma unroll
       for (int n = 0; n < NO; ++n) acc[mt][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      for (int k = 0; k < parts.count; ++k) {
-        const uint64_t both = __hip_atomic_load(ml_at(k, mt), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const float mk = __uint_as_float(static_cast<uint32_t>(both)), lk = __uint_as_float(static_cast<uint32_t>(both >> 32));
+    }
+    for (int k = 0; k < parts.count; ++k) {
+      uint64_t both[kRowTiles];
+      u32x4_t y[kRowTiles][NO];  // all of a part is in flight at once
+#pragma unroll
+      for (int mt = 0; mt < kRowTiles; ++mt) {
+        both[mt] = __hip_atomic_load(ml_at(k, mt), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (int n = 0; n < NO; ++n) y[mt][n] = __builtin_amdgcn_raw_buffer_load_b128(o_rsrc, place(k, mt, n), 0, kAgentScope);
+      }
+#pragma unroll
+      for (int mt = 0; mt < kRowTiles; ++mt) {
+        const float mk = __uint_as_float(static_cast<uint32_t>(both[mt])), lk = __uint_as_float(static_cast<uint32_t>(both[mt] >> 32));
         const float t_new = fmaxf(m[mt], mk), f = __builtin_amdgcn_exp2f(m[mt] - t_new), fk = __builtin_amdgcn_exp2f(mk - t_new);
         m[mt] = t_new;
         l[mt] = l[mt] * f + lk * fk;
 #pragma unroll
-        for (int n = 0; n < NO; ++n) {
-          const f32x4_t y = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(o_rsrc, place(k, mt, n), 0, kAgentScope));
-          acc[mt][n] = acc[mt][n] * f + y * fk;
-        }
+        for (int n = 0; n < NO; ++n) acc[mt][n] = acc[mt][n] * f + __builtin_bit_cast(f32x4_t, y[mt][n]) * fk;
       }
     }
   }
@@ -729,11 +779,14 @@ __device__ __forceinline__ int place_in_cut(int b, int n) {
 struct Run {
   Cut cut;
   int self, seq, n;
+  int fixed;  // first stream: positions of every item, 0 where they are its keys and kThinPad
+  Seq first;  // lengths of sequence `seq`
   int64_t x, x_end, off;
 };
 
 struct SchedLds {
   int64_t sums[4][2];
+  int seqs[4], longest[4];
   Run run[2];
   int flag;
 };
@@ -757,7 +810,8 @@ __device__ __forceinline__ int64_t uniform(int64_t x) {
   return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 __device__ __forceinline__ Run uniform(const Run& r) {
-  return {{uniform(r.cut.total), uniform(r.cut.n)}, uniform(r.self), uniform(r.seq), uniform(r.n), uniform(r.x), uniform(r.x_end), uniform(r.off)};
+  return {{uniform(r.cut.per_unit), uniform(r.cut.rest), uniform(r.cut.n), uniform(r.cut.block), uniform(r.cut.pair), uniform(r.cut.lead)}, uniform(r.self), uniform(r.seq), uniform(r.n), uniform(r.fixed),
+          {uniform(r.first.q0), uniform(r.first.q_len), uniform(r.first.kv_len)}, uniform(r.x), uniform(r.x_end), uniform(r.off)};
 }
 
 // The two streams are functions of their own, so that the registers of one loop are not shared out by the other's.
@@ -769,13 +823,12 @@ __device__ __attribute__((noinline)) void thin_phase(uint64_t args) {
   Window window;
   int s = run.seq;
   int64_t off = run.off, x = run.x;
+  Seq q = run.first;
   while (x < run.x_end && s < run.n) {
-    window.at(a, run.n, s);
-    const Seq q = window.get(s);
-    const int keys = thin_keys(a, q), len = keys + kThinPad;
+    const int keys = thin_keys(a, q), len = run.fixed > 0 ? run.fixed : keys + kThinPad;
     const Range range = key_range(a, q, 0, q.q_len);
     const int all = range.end - (range.first & ~31);  // keys as they are walked
-    int h = static_cast<int>(off / len);
+    int h = static_cast<int>(divide(off, len));
     int begin = static_cast<int>(off - static_cast<int64_t>(h) * len);
     for (; h < a.p.num_kv_heads && x < run.x_end; ++h, begin = 0) {
       const int end = static_cast<int>(min(static_cast<int64_t>(len), begin + (run.x_end - x)));
@@ -785,7 +838,8 @@ __device__ __attribute__((noinline)) void thin_phase(uint64_t args) {
       x += end - begin;
     }
     off = 0;
-    s = window.next(a, run.n, s + 1, true);
+    if (x < run.x_end) s = window.next(a, run.n, s + 1, true);
+    if (x < run.x_end && s < run.n) q = window.get(s);
   }
 }
 
@@ -799,12 +853,11 @@ __device__ __attribute__((noinline)) void tile_phase(uint64_t args) {
   int s = run.seq;
   int64_t off = run.off, x = run.x;
   const int heads = a.p.num_kv_heads * a.subs;
+  Seq q = run.first;
   while (x < run.x_end && s < run.n) {
-    window.at(a, run.n, s);
-    const Seq q = window.get(s);
     const int tiles = tiles_of(a, q);
     const int64_t len = tiles_before(a, q, tiles, true);
-    int h = static_cast<int>(off / len);
+    int h = static_cast<int>(divide(off, len));
     int64_t rest = off - static_cast<int64_t>(h) * len;
     int tile = 0;
     for (int hi = tiles; hi - tile > 1;) {  // the last tile that starts at or before the position
@@ -820,12 +873,13 @@ __device__ __attribute__((noinline)) void tile_phase(uint64_t args) {
         const int end = static_cast<int>(min(static_cast<int64_t>(item), begin + (run.x_end - x)));
         const int ka = begin >= keys ? all : begin / kStep * kStep, kb = end >= keys ? all : end / kStep * kStep;
         if (ka < kb || (keys == 0 && begin == 0))
-          tile_item<kCode, D, T, kParts, kCap, kWide>(a, q, s, h, tile, keys == 0 ? 0 : ka, kb, run.cut, run.self, x - begin, &lds.sched.flag);
+          tile_item<kCode, D, T, kParts, kCap, kWide>(a, q, s, h, tile, keys == 0 ? 0 : ka, kb, run.cut, run.self, x - begin);
         x += end - begin;
       }
     }
     off = 0;
-    s = window.next(a, run.n, s + 1, false);
+    if (x < run.x_end) s = window.next(a, run.n, s + 1, false);
+    if (x < run.x_end && s < run.n) q = window.get(s);
   }
 }
 
@@ -836,41 +890,68 @@ __global__ __launch_bounds__(256, 2) void quant_attention_kernel(QuantArgs) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n = min(max(a.p.num_seqs[0], 0), a.p.max_num_seqs);
 
-  // Lengths of the two streams.
-  const int per = (n + 255) >> 8;
-  const int s0 = min(static_cast<int>(threadIdx.x) * per, n), s1 = min(s0 + per, n);
+  // Lengths of the two streams; of the first also the longest item and how many there are.
+  const int per = (a.p.max_num_seqs + 255) >> 8;
+  const int s0 = min(static_cast<int>(threadIdx.x) * per, a.p.max_num_seqs), s1 = min(s0 + per, a.p.max_num_seqs);
   auto length = [&](const Seq& q, bool thin) {
     return thin ? static_cast<int64_t>(thin_keys(a, q) + kThinPad) * a.p.num_kv_heads : tiles_before(a, q, tiles_of(a, q), true) * a.p.num_kv_heads * a.subs;
   };
   int64_t sum[2] = {0, 0};
+  int seqs = 0, longest = 0;
+  Seq only = {0, 0, 0};
   for (int s = s0; s < s1; ++s) {
     const Seq q = load_seq(a, n, s);
+    only = q;
     if (q.q_len == 0) continue;
     const bool thin = is_thin(a, q);
     sum[thin ? 0 : 1] += length(q, thin);
+    if (thin) ++seqs, longest = max(longest, thin_keys(a, q));
   }
   int64_t inc[2] = {sum[0], sum[1]};
+  int seqs_inc = seqs;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const int64_t x = __shfl_up(inc[0], o), y = __shfl_up(inc[1], o);
-    if (lane >= o) inc[0] += x, inc[1] += y;
+    const int z = __shfl_up(seqs_inc, o);
+    if (lane >= o) inc[0] += x, inc[1] += y, seqs_inc += z;
+    longest = max(longest, __shfl_xor(longest, o));
   }
-  if (lane == 63) sched.sums[wave][0] = inc[0], sched.sums[wave][1] = inc[1];
+  if (lane == 63) {
+    sched.sums[wave][0] = inc[0], sched.sums[wave][1] = inc[1];
+    sched.seqs[wave] = seqs_inc, sched.longest[wave] = longest;
+  }
   __syncthreads();
   int64_t before[2] = {inc[0] - sum[0], inc[1] - sum[1]}, total[2] = {0, 0};
+  int seqs_before = seqs_inc - seqs, seqs_all = 0;
+  longest = 0;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    if (w < wave) before[0] += sched.sums[w][0], before[1] += sched.sums[w][1];
+    if (w < wave) before[0] += sched.sums[w][0], before[1] += sched.sums[w][1], seqs_before += sched.seqs[w];
     total[0] += sched.sums[w][0], total[1] += sched.sums[w][1];
+    seqs_all += sched.seqs[w];
+    longest = max(longest, sched.longest[w]);
+  }
+  // Few short items: a workgroup each, so that none is cut and no state goes through memory.
+  const int64_t items = static_cast<int64_t>(seqs_all) * a.p.num_kv_heads;
+  const int fixed = items <= a.grid / 2 && longest <= kThinWhole ? longest + kThinPad : 0;
+  if (fixed > 0) {
+    sum[0] = static_cast<int64_t>(seqs) * a.p.num_kv_heads * fixed;
+    before[0] = static_cast<int64_t>(seqs_before) * a.p.num_kv_heads * fixed;
+    total[0] = items * fixed;
   }
   bool has[2];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     Run r;
-    r.seq = 0, r.off = 0;
     r.n = n;
-    r.cut.total = total[c];
-    r.cut.n = static_cast<int>(min(static_cast<int64_t>(a.grid), max(total[c] / (c == 0 ? kThinLeast : kTileLeast), static_cast<int64_t>(1))));
+    r.fixed = c == 0 ? fixed : 0;
+    const int64_t most = max(total[c] / (c == 0 ? kThinLeast : kTileLeast), static_cast<int64_t>(1));  // workgroups worth their while
+    const bool whole = most >= a.grid && r.fixed == 0;
+    r.cut.n = whole ? a.grid : static_cast<int>(r.fixed > 0 ? items : min(most, static_cast<int64_t>(a.grid / 2)));
+    r.cut.block = whole ? a.grid / 8 : 2 * r.cut.n;
+    r.cut.pair = whole ? kPairUnits : 2;
+    r.cut.lead = !whole ? 1 : c == 0 ? kFirstThin : kPairUnits - kFirstTile;
+    r.cut.set(total[c]);
     // the first stream from the grid's front, the second from its back: where both are short they meet different workgroups
     r.self = total[c] > 0 ? place_in_cut(c == 0 ? blockIdx.x : a.grid - 1 - blockIdx.x, r.cut.n) : -1;
     r.x = r.self >= 0 ? r.cut.bound(r.self) : 0;
@@ -880,11 +961,12 @@ __global__ __launch_bounds__(256, 2) void quant_attention_kernel(QuantArgs) {
     if (r.self >= 0 && r.x >= before[c] && r.x < before[c] + sum[c]) {
       int64_t off = r.x - before[c];
       for (int s = s0; s < s1; ++s) {
-        const Seq q = load_seq(a, n, s);
+        const Seq q = per == 1 ? only : load_seq(a, n, s);
         if (q.q_len == 0 || is_thin(a, q) != (c == 0)) continue;
-        const int64_t len = length(q, c == 0);
+        const int64_t len = r.fixed > 0 ? static_cast<int64_t>(r.fixed) * a.p.num_kv_heads : length(q, c == 0);
         if (off < len) {
           r.seq = s;
+          r.first = q;
           r.off = off;
           sched.run[c] = r;
           break;

@@ -17,7 +17,7 @@ int tile_rows(const RpaQuantParams& p) {
     default: return 64 * (f32 ? quant_row_tiles<256, 3>() : quant_row_tiles<256, 1>());
   }
 }
-int grid_of() { return std::max(8, 2 * device_cu_count() / 8 * 8); }  // two workgroups per compute unit, the same number on each XCD
+int grid_of() { return std::max(16, 2 * device_cu_count() / 16 * 16); }  // two workgroups per compute unit, the same number on each XCD
 
 struct Layout {
   uint64_t thin_o, thin_ml, tile_o, tile_ml, total;

@@ -36,19 +36,19 @@ class BuildBlockTables:
 
     op_id = "build_block_tables"
 
+    _entry = _native.Entry("rpa_block_tables_launch", _native.RpaBlockTablesParams)
+
     def run(self, query_lens, cached_lens, block_tables, free_pages, free_state, num_seqs, *, page_size: int, total_tokens: int):
         if block_tables.dim() != 2 or 0 in block_tables.shape:
             raise ValueError(f"block_tables must be [max_num_seqs, pages_per_seq], got {tuple(block_tables.shape)}")
         n, pages_per_seq = block_tables.shape
-        for name, t, shape in (("query_lens", query_lens, (n,)), ("cached_lens", cached_lens, (n,)), ("free_state", free_state, (2,))):
-            if tuple(t.shape) != shape:
-                raise ValueError(f"{name}.shape={tuple(t.shape)} must be {shape}")
-        if free_pages.dim() != 1 or free_pages.numel() == 0:
-            raise ValueError(f"free_pages must be a ring of one page at least, got {tuple(free_pages.shape)}")
         if not isinstance(num_seqs, torch.Tensor):
             num_seqs = torch.tensor([int(num_seqs)], dtype=torch.int32, device=block_tables.device)
-        elif tuple(num_seqs.shape) != (1,):
-            raise ValueError(f"num_seqs.shape={tuple(num_seqs.shape)} must be (1,)")
+        for name, t, length in (("query_lens", query_lens, n), ("cached_lens", cached_lens, n), ("free_state", free_state, 2), ("num_seqs", num_seqs, 1)):
+            if t.dim() != 1 or t.shape[0] != length:
+                raise ValueError(f"{name}.shape={tuple(t.shape)} must be ({length},)")
+        if free_pages.dim() != 1 or free_pages.shape[0] == 0:
+            raise ValueError(f"free_pages must be a ring of one page at least, got {tuple(free_pages.shape)}")
         for name, t in (("query_lens", query_lens), ("cached_lens", cached_lens), ("block_tables", block_tables),
                         ("free_pages", free_pages), ("free_state", free_state), ("num_seqs", num_seqs)):
             if t.dtype != torch.int32:
@@ -59,24 +59,21 @@ class BuildBlockTables:
             raise ValueError(f"page_size={page_size} must be positive and below 2**31")
         if not 0 <= total_tokens < 2**31:
             raise ValueError(f"total_tokens={total_tokens} must be from 0 to 2**31 - 1")
-        dev = _on_device("build_block_tables", block_tables, query_lens=query_lens, cached_lens=cached_lens,
-                         free_pages=free_pages, free_state=free_state, num_seqs=num_seqs)
+        index = _on_device("build_block_tables", block_tables, query_lens=query_lens, cached_lens=cached_lens,
+                           free_pages=free_pages, free_state=free_state, num_seqs=num_seqs)
         query_lens, cached_lens, free_state = query_lens.contiguous(), cached_lens.contiguous(), free_state.contiguous()
 
-        # one allocation, one view for each result; the kernels' scratch first, at the allocator's alignment
+        # one allocation: the kernels' scratch, at the allocator's alignment, and a view for each result
         sizes = (4 * n + 4, n + 1, n, total_tokens, total_tokens, n, n, 2)
-        scratch, *views = torch.empty(sum(sizes), dtype=torch.int32, device=dev).split(sizes)
-        r = BlockTables(*views)
-        p = _native.RpaBlockTablesParams()
-        p.query_lens, p.cached_lens, p.block_tables = query_lens.data_ptr(), cached_lens.data_ptr(), block_tables.data_ptr()
-        p.free_pages, p.free_state, p.num_seqs = free_pages.data_ptr(), free_state.data_ptr(), num_seqs.data_ptr()
-        p.query_start_loc, p.context_lens, p.slot_mapping = r.query_start_loc.data_ptr(), r.context_lens.data_ptr(), r.slot_mapping.data_ptr()
-        p.positions, p.admitted, p.cached_lens_out = r.positions.data_ptr(), r.admitted.data_ptr(), r.cached_lens.data_ptr()
-        p.free_state_out, p.scratch = r.free_state.data_ptr(), scratch.data_ptr()
-        p.max_num_seqs, p.pages_per_seq, p.num_free_slots = n, pages_per_seq, free_pages.numel()
-        p.page_size, p.total_tokens = page_size, total_tokens
-        _call("rpa_block_tables_launch", p, dev)
-        return r
+        memory = torch.empty(sum(sizes), dtype=torch.int32, device=block_tables.device)
+        results = memory.split(sizes)[1:]
+        at, places = memory.data_ptr(), []
+        for size in sizes:
+            places.append(at)
+            at += 4 * size
+        _call(self._entry, index, query_lens.data_ptr(), cached_lens.data_ptr(), block_tables.data_ptr(), free_pages.data_ptr(), free_state.data_ptr(),
+              num_seqs.data_ptr(), *places[1:], places[0], n, pages_per_seq, free_pages.shape[0], page_size, total_tokens, 0)
+        return BlockTables._make(results)
 
 
 _build = BuildBlockTables()

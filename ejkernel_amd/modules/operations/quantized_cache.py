@@ -15,8 +15,6 @@ The attention over it is ``quantized_ragged_page_attention``.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from ... import _native
@@ -28,90 +26,94 @@ _CACHE_DTYPES = {torch.int8: _native.RPA_DTYPE_INT8, torch.float8_e4m3fn: _nativ
 _VALUE_DTYPES = {torch.bfloat16: _native.RPA_DTYPE_BF16, torch.float32: _native.RPA_DTYPE_F32}
 
 
-def _check_cache(kv_cache, kv_scales) -> int:
-    """Checks the two arrays against each other; returns the tokens a scale covers."""
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: torch.cuda.current_stream builds an object around it
+_current_device = torch._C._cuda_getDevice
+
+
+def _check_cache(kv_cache, kv_scales) -> tuple[int, int, int, int, int, int]:
+    """Checks the two arrays against each other; returns the shape of the cache, the tokens a scale covers and the type's code."""
     if kv_cache.dim() != 4:
         raise ValueError(f"kv_cache must be [num_pages, 2 * num_kv_heads, page_size, head_dim], got {tuple(kv_cache.shape)}")
-    if kv_cache.dtype not in _CACHE_DTYPES:
+    code = _CACHE_DTYPES.get(kv_cache.dtype)
+    if code is None:
         raise ValueError(f"kv_cache.dtype={kv_cache.dtype} must be int8, float8_e4m3fn or float8_e5m2")
-    num_pages, heads, page_size, _ = kv_cache.shape
+    num_pages, heads, page_size, head_dim = kv_cache.shape
     if heads % 2 != 0 or heads == 0:
         raise ValueError(f"kv_cache.shape[1]={heads} must be 2 * num_kv_heads")
-    if kv_scales.dim() != 3 or kv_scales.dtype != torch.float32 or kv_scales.shape[0] != num_pages or kv_scales.shape[1] != heads:
-        raise ValueError(f"kv_scales must be float32 [{num_pages}, {heads}, page_size // block], got {kv_scales.dtype} {tuple(kv_scales.shape)}")
-    blocks = kv_scales.shape[2]
+    shape = kv_scales.shape
+    if len(shape) != 3 or kv_scales.dtype != torch.float32 or shape[0] != num_pages or shape[1] != heads:
+        raise ValueError(f"kv_scales must be float32 [{num_pages}, {heads}, page_size // block], got {kv_scales.dtype} {tuple(shape)}")
+    blocks = shape[2]
     if blocks == 0 or page_size % blocks != 0:
         raise ValueError(f"kv_scales.shape[2]={blocks} must divide page_size={page_size}")
     if not kv_cache.is_contiguous() or not kv_scales.is_contiguous():
         raise ValueError("kv_cache and kv_scales must be contiguous")
-    return page_size // blocks
+    return num_pages, heads, page_size, head_dim, page_size // blocks, code
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``[tokens, heads, head_dim]`` as the kernels read it in place: rows of 16-byte pieces; anything else is copied."""
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """``[tokens, heads, head_dim]`` as the kernels read it in place, rows of 16-byte pieces, with its strides between tokens
+    and heads; anything else is copied."""
     unit = 16 // t.element_size()
-    if t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(t.shape[k] <= 1 or t.stride(k) % unit == 0 for k in (0, 1)):
-        return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    for _ in range(3):
+        token, head, element = t.stride()
+        if t.shape[0] <= 1:
+            token = 0
+        if t.shape[1] <= 1:
+            head = 0
+        if element == 1 and token % unit == 0 and head % unit == 0 and t.data_ptr() % 16 == 0:
+            break
+        t = t.clone() if t.is_contiguous() else t.contiguous()
+    return t, token, head
 
 
-def _strides(t: torch.Tensor) -> tuple[int, int]:
-    return (t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
-
-
-def _on_device(op: str, first: torch.Tensor, **others: torch.Tensor) -> torch.device:
+def _on_device(op: str, first: torch.Tensor, **others: torch.Tensor) -> int:
+    """Index of the device that all of the tensors are on."""
     if not first.is_cuda:
         raise RuntimeError(f"{op} needs tensors on a ROCm device (gfx950); there is no CPU implementation in this package.")
-    dev = first.device
+    index = first.get_device()
     for name, t in others.items():
-        if t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, expected {dev}")
-    return dev
+        if t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, expected {first.device}")
+    return index
 
 
-def _call(entry: str, params, dev: torch.device) -> None:
-    """Calls a C entry point on the current stream of ``dev``."""
-    fn = getattr(_native.load(), entry)
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(ctypes.byref(params), torch.cuda.current_stream(dev).cuda_stream)
+def _call(entry: _native.Entry, index: int, *values) -> None:
+    """Calls a C entry point on the current stream of device ``index``."""
+    if _current_device() == index:
+        entry(_raw_stream(index), *values)
     else:
-        with torch.cuda.device(dev):
-            rc = fn(ctypes.byref(params), torch.cuda.current_stream(dev).cuda_stream)
-    if rc != 0:
-        kind = ValueError if rc in (-1, -2) else RuntimeError
-        raise kind(f"{entry} refused the call ({rc}): {_native.last_error()}")
+        with torch.cuda.device(index):
+            entry(_raw_stream(index), *values)
 
 
 class QuantizedCacheUpdate:
     """Kernel object of ``quantized_cache_update``."""
 
     op_id = "quantized_cache_update"
+    _entry = _native.Entry("rpa_quant_update_launch", _native.RpaQuantUpdateParams)
 
     def run(self, keys, values, kv_cache, kv_scales, slot_mapping):
-        block = _check_cache(kv_cache, kv_scales)
-        num_pages, heads, page_size, head_dim = kv_cache.shape
-        if keys.dim() != 3 or keys.shape != values.shape or keys.shape[1] != heads // 2 or keys.shape[2] != head_dim:
-            raise ValueError(f"keys and values must be [total_tokens, {heads // 2}, {head_dim}], got {tuple(keys.shape)} and {tuple(values.shape)}")
-        if keys.dtype not in _VALUE_DTYPES or values.dtype != keys.dtype:
+        num_pages, heads, page_size, head_dim, block, code = _check_cache(kv_cache, kv_scales)
+        shape = keys.shape
+        if len(shape) != 3 or shape != values.shape or shape[1] != heads // 2 or shape[2] != head_dim:
+            raise ValueError(f"keys and values must be [total_tokens, {heads // 2}, {head_dim}], got {tuple(shape)} and {tuple(values.shape)}")
+        dtype = _VALUE_DTYPES.get(keys.dtype)
+        if dtype is None or values.dtype != keys.dtype:
             raise ValueError(f"keys and values must share one dtype, bfloat16 or float32, got {keys.dtype} and {values.dtype}")
-        if tuple(slot_mapping.shape) != (keys.shape[0],) or slot_mapping.dtype != torch.int32:
-            raise ValueError(f"slot_mapping must be int32 [{keys.shape[0]}], got {slot_mapping.dtype} {tuple(slot_mapping.shape)}")
-        if any(t.requires_grad for t in (keys, values, kv_scales)):
+        tokens = shape[0]
+        if slot_mapping.dim() != 1 or slot_mapping.shape[0] != tokens or slot_mapping.dtype != torch.int32:
+            raise ValueError(f"slot_mapping must be int32 [{tokens}], got {slot_mapping.dtype} {tuple(slot_mapping.shape)}")
+        if keys.requires_grad or values.requires_grad or kv_scales.requires_grad:
             raise NotImplementedError("quantized_cache_update is forward-only; detach the inputs")
-        dev = _on_device("quantized_cache_update", kv_cache, keys=keys, values=values, kv_scales=kv_scales, slot_mapping=slot_mapping)
-        if keys.shape[0] == 0:
+        index = _on_device("quantized_cache_update", kv_cache, keys=keys, values=values, kv_scales=kv_scales, slot_mapping=slot_mapping)
+        if tokens == 0:
             return kv_cache, kv_scales
-        keys, values, slot_mapping = _rows(keys), _rows(values), slot_mapping.contiguous()
-        p = _native.RpaQuantUpdateParams()
-        p.keys, p.values = keys.data_ptr(), values.data_ptr()
-        p.kv_cache, p.kv_scales, p.slot_mapping = kv_cache.data_ptr(), kv_scales.data_ptr(), slot_mapping.data_ptr()
-        p.key_token_stride, p.key_head_stride = _strides(keys)
-        p.value_token_stride, p.value_head_stride = _strides(values)
-        p.total_tokens, p.num_kv_heads, p.head_dim = keys.shape[0], heads // 2, head_dim
-        p.page_size, p.scale_block, p.num_pages = page_size, block, num_pages
-        p.dtype, p.cache_dtype = _VALUE_DTYPES[keys.dtype], _CACHE_DTYPES[kv_cache.dtype]
-        _call("rpa_quant_update_launch", p, dev)
+        keys, key_token, key_head = _rows(keys)
+        values, value_token, value_head = _rows(values)
+        slot_mapping = slot_mapping.contiguous()
+        _call(self._entry, index, keys.data_ptr(), values.data_ptr(), kv_cache.data_ptr(), kv_scales.data_ptr(), slot_mapping.data_ptr(),
+              key_token, key_head, value_token, value_head, tokens, heads // 2, head_dim, page_size, block, num_pages, dtype, code)
         return kv_cache, kv_scales
 
 
@@ -119,30 +121,27 @@ class QuantizedCacheGather:
     """Kernel object of ``quantized_cache_gather``."""
 
     op_id = "quantized_cache_gather"
+    _entry = _native.Entry("rpa_quant_gather_launch", _native.RpaQuantGatherParams)
 
     def run(self, kv_cache, kv_scales, slot_mapping, *, dtype: torch.dtype = torch.bfloat16):
-        block = _check_cache(kv_cache, kv_scales)
-        num_pages, heads, page_size, head_dim = kv_cache.shape
-        if dtype not in _VALUE_DTYPES:
+        num_pages, heads, page_size, head_dim, block, code = _check_cache(kv_cache, kv_scales)
+        kind = _VALUE_DTYPES.get(dtype)
+        if kind is None:
             raise ValueError(f"dtype={dtype} must be bfloat16 or float32")
         if slot_mapping.dim() != 1 or slot_mapping.dtype != torch.int32:
             raise ValueError(f"slot_mapping must be int32 [total_tokens], got {slot_mapping.dtype} {tuple(slot_mapping.shape)}")
         if kv_scales.requires_grad:
             raise NotImplementedError("quantized_cache_gather is forward-only; detach the inputs")
-        dev = _on_device("quantized_cache_gather", kv_cache, kv_scales=kv_scales, slot_mapping=slot_mapping)
+        index = _on_device("quantized_cache_gather", kv_cache, kv_scales=kv_scales, slot_mapping=slot_mapping)
         tokens = slot_mapping.shape[0]
-        keys = torch.empty((tokens, heads // 2, head_dim), dtype=dtype, device=dev)
-        values = torch.empty_like(keys)
+        shape = (tokens, heads // 2, head_dim)
+        keys = torch.empty(shape, dtype=dtype, device=kv_cache.device)
+        values = torch.empty(shape, dtype=dtype, device=kv_cache.device)
         if tokens == 0:
             return keys, values
         slot_mapping = slot_mapping.contiguous()
-        p = _native.RpaQuantGatherParams()
-        p.kv_cache, p.kv_scales, p.slot_mapping = kv_cache.data_ptr(), kv_scales.data_ptr(), slot_mapping.data_ptr()
-        p.keys, p.values = keys.data_ptr(), values.data_ptr()
-        p.total_tokens, p.num_kv_heads, p.head_dim = tokens, heads // 2, head_dim
-        p.page_size, p.scale_block, p.num_pages = page_size, block, num_pages
-        p.dtype, p.cache_dtype = _VALUE_DTYPES[dtype], _CACHE_DTYPES[kv_cache.dtype]
-        _call("rpa_quant_gather_launch", p, dev)
+        _call(self._entry, index, kv_cache.data_ptr(), kv_scales.data_ptr(), slot_mapping.data_ptr(), keys.data_ptr(), values.data_ptr(),
+              tokens, heads // 2, head_dim, page_size, block, num_pages, kind, code)
         return keys, values
 
 

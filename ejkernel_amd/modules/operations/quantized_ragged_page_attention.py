@@ -9,46 +9,51 @@ probability and value scale are rounded, to bfloat16 (with float32 queries not e
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from ... import _native
 from .configs import QuantizedRaggedPageAttentionConfig
-from .quantized_cache import _CACHE_DTYPES, _VALUE_DTYPES, _call, _check_cache, _on_device, _rows, _strides
+from .quantized_cache import _VALUE_DTYPES, _call, _check_cache, _current_device, _on_device, _raw_stream, _rows
 from .ragged_page_attention import _call_workspace, _sinks_per_q_head
 
 __all__ = ["QuantizedRaggedPageAttention", "quantized_ragged_page_attention"]
+
+
+_sizes: dict[tuple[int, int, int], int] = {}  # workspace bytes by device, dtype and head_dim, all that they depend on
 
 
 class QuantizedRaggedPageAttention:
     """Kernel object of ``quantized_ragged_page_attention``."""
 
     op_id = "quantized_ragged_page_attention"
+    _entry = _native.Entry("rpa_quant_fwd_launch", _native.RpaQuantParams)
 
     def run(self, queries, kv_cache, kv_scales, context_lens, block_tables, query_start_loc, num_seqs, softmax_aux=None, *,
             softmax_scale: float | None = None, logits_soft_cap: float | None = None, sliding_window: int | None = None,
             cfg: QuantizedRaggedPageAttentionConfig):
         cfg.validate()
-        block = _check_cache(kv_cache, kv_scales)
-        num_pages, heads, page_size, head_dim = kv_cache.shape
+        num_pages, heads, page_size, head_dim, block, code = _check_cache(kv_cache, kv_scales)
         num_kv_heads = heads // 2
-        if queries.dim() != 3 or queries.shape[2] != head_dim:
-            raise ValueError(f"queries must be [total_tokens, num_q_heads, {head_dim}], got {tuple(queries.shape)}")
-        if queries.dtype not in _VALUE_DTYPES:
+        shape = queries.shape
+        if len(shape) != 3 or shape[2] != head_dim:
+            raise ValueError(f"queries must be [total_tokens, num_q_heads, {head_dim}], got {tuple(shape)}")
+        dtype = _VALUE_DTYPES.get(queries.dtype)
+        if dtype is None:
             raise ValueError(f"queries.dtype={queries.dtype} must be bfloat16 or float32")
-        total_tokens, num_q_heads, _ = queries.shape
+        total_tokens, num_q_heads, _ = shape
         if num_q_heads == 0 or num_q_heads % num_kv_heads != 0:
             raise ValueError(f"{num_q_heads=} must be divisible by {num_kv_heads=}")
         if block_tables.dim() != 2 or 0 in block_tables.shape:
             raise ValueError(f"block_tables must be [max_num_seqs, pages_per_seq], got {tuple(block_tables.shape)}")
         max_num_seqs, pages_per_seq = block_tables.shape
-        if tuple(context_lens.shape) != (max_num_seqs,):
-            raise ValueError(f"context_lens.shape={tuple(context_lens.shape)} must be ({max_num_seqs},)")
-        if tuple(query_start_loc.shape) != (max_num_seqs + 1,):
-            raise ValueError(f"query_start_loc.shape={tuple(query_start_loc.shape)} must be ({max_num_seqs + 1},)")
         if not isinstance(num_seqs, torch.Tensor):
             num_seqs = torch.tensor([int(num_seqs)], dtype=torch.int32, device=queries.device)
-        elif tuple(num_seqs.shape) != (1,):
-            raise ValueError(f"num_seqs.shape={tuple(num_seqs.shape)} must be (1,)")
+        for name, t, length in (("context_lens", context_lens, max_num_seqs), ("query_start_loc", query_start_loc, max_num_seqs + 1),
+                                ("num_seqs", num_seqs, 1)):
+            if t.dim() != 1 or t.shape[0] != length:
+                raise ValueError(f"{name}.shape={tuple(t.shape)} must be ({length},)")
         for name, t in (("context_lens", context_lens), ("block_tables", block_tables), ("query_start_loc", query_start_loc),
                         ("num_seqs", num_seqs)):
             if t.dtype != torch.int32:
@@ -57,34 +62,46 @@ class QuantizedRaggedPageAttention:
             raise ValueError(f"{sliding_window=} must be positive.")
         if logits_soft_cap is not None and logits_soft_cap == 0.0:
             raise ValueError(f"{logits_soft_cap=} must not be 0.0.")
-        if any(t.requires_grad for t in (queries, kv_scales)):
+        if queries.requires_grad or kv_scales.requires_grad:
             raise NotImplementedError("quantized_ragged_page_attention is forward-only; detach the inputs")
-        dev = _on_device("quantized_ragged_page_attention", queries, kv_cache=kv_cache, kv_scales=kv_scales, context_lens=context_lens,
-                         block_tables=block_tables, query_start_loc=query_start_loc, num_seqs=num_seqs)
-        out = torch.empty(queries.shape, dtype=queries.dtype, device=dev)
+        index = _on_device("quantized_ragged_page_attention", queries, kv_cache=kv_cache, kv_scales=kv_scales, context_lens=context_lens,
+                           block_tables=block_tables, query_start_loc=query_start_loc, num_seqs=num_seqs)
+        if _current_device() != index:
+            with torch.cuda.device(index):
+                return self.run(queries, kv_cache, kv_scales, context_lens, block_tables, query_start_loc, num_seqs, softmax_aux,
+                                softmax_scale=softmax_scale, logits_soft_cap=logits_soft_cap, sliding_window=sliding_window, cfg=cfg)
+        out = torch.empty(shape, dtype=queries.dtype, device=queries.device)
         if total_tokens == 0:
             return out
-        queries = _rows(queries)
+        queries, token_stride, head_stride = _rows(queries)
         context_lens, block_tables, query_start_loc = context_lens.contiguous(), block_tables.contiguous(), query_start_loc.contiguous()
-        p = _native.RpaQuantParams()
+        sinks = None
         if softmax_aux is not None and softmax_aux.shape[-1] > 0:
-            sinks = _sinks_per_q_head(softmax_aux.to(dev), num_q_heads, num_kv_heads)
-            p.sinks, p.num_sinks = sinks.data_ptr(), sinks.shape[1]
-        p.queries, p.kv_cache, p.kv_scales = queries.data_ptr(), kv_cache.data_ptr(), kv_scales.data_ptr()
-        p.context_lens, p.block_tables = context_lens.data_ptr(), block_tables.data_ptr()
-        p.query_start_loc, p.num_seqs, p.out = query_start_loc.data_ptr(), num_seqs.data_ptr(), out.data_ptr()
-        p.query_token_stride, p.query_head_stride = _strides(queries)
-        p.total_tokens, p.num_q_heads, p.num_kv_heads, p.head_dim = total_tokens, num_q_heads, num_kv_heads, head_dim
-        p.page_size, p.scale_block, p.num_pages = page_size, block, num_pages
-        p.max_num_seqs, p.pages_per_seq = max_num_seqs, pages_per_seq
-        p.softmax_scale = head_dim**-0.5 if softmax_scale is None else softmax_scale
-        p.logits_soft_cap = 0.0 if logits_soft_cap is None else logits_soft_cap
-        p.sliding_window = 0 if sliding_window is None else min(sliding_window, 2**31 - 1)
-        p.dtype, p.cache_dtype = _VALUE_DTYPES[queries.dtype], _CACHE_DTYPES[kv_cache.dtype]
-        workspace = _call_workspace(dev, p, "rpa_quant_workspace_bytes")
-        p.workspace, p.workspace_bytes = workspace.data_ptr(), workspace.numel()
-        _call("rpa_quant_fwd_launch", p, dev)
+            sinks = _sinks_per_q_head(softmax_aux.to(queries.device), num_q_heads, num_kv_heads)
+        size = _sizes.get((index, dtype, head_dim))
+        if size is None:
+            size = self._workspace_bytes(index, dtype, head_dim)
+        workspace = _call_workspace(queries.device, size, _raw_stream(index))
+        _call(self._entry, index, queries.data_ptr(), kv_cache.data_ptr(), kv_scales.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(),
+              query_start_loc.data_ptr(), num_seqs.data_ptr(), 0 if sinks is None else sinks.data_ptr(), out.data_ptr(),
+              workspace.data_ptr(), workspace.numel(), token_stride, head_stride, total_tokens, num_q_heads, num_kv_heads, head_dim, page_size, block,
+              num_pages, max_num_seqs, pages_per_seq, 0 if sinks is None else sinks.shape[1],
+              head_dim**-0.5 if softmax_scale is None else softmax_scale, 0.0 if logits_soft_cap is None else logits_soft_cap,
+              0 if sliding_window is None else min(sliding_window, 2**31 - 1), dtype, code, 0)
         return out
+
+    @staticmethod
+    def _workspace_bytes(index: int, dtype: int, head_dim: int) -> int:
+        """Asks the library once per device, dtype and head_dim; other dims do not enter the size."""
+        p = _native.RpaQuantParams()
+        p.num_q_heads = p.num_kv_heads = p.num_pages = p.max_num_seqs = p.pages_per_seq = 1
+        p.page_size = p.scale_block = 16
+        p.head_dim, p.dtype, p.cache_dtype = head_dim, dtype, _native.RPA_DTYPE_INT8
+        size = int(_native.load().rpa_quant_workspace_bytes(ctypes.byref(p)))
+        if size == 0:
+            raise ValueError(_native.last_error())
+        _sizes[(index, dtype, head_dim)] = size
+        return size
 
     def heuristic_cfg(self, inv=None) -> QuantizedRaggedPageAttentionConfig:
         """The work is cut on the device; there is nothing to choose."""

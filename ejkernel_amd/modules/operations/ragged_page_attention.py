@@ -156,23 +156,20 @@ def _workspace(device: torch.device, nbytes: int, stream_ptr: int) -> torch.Tens
     return ws
 
 
-def _call_workspace(dev: torch.device, params, size_entry: str) -> torch.Tensor:
-    """Cleared workspace for one call on the current stream of ``dev``.
+_TICKET_BYTES = 1 << 16  # the tickets of the operations that use _call_workspace lie in the first 64 KiB
+
+
+def _call_workspace(dev: torch.device, nbytes: int, stream_ptr: int) -> torch.Tensor:
+    """Cleared workspace for one call on the current stream of ``dev``, the current device.
 
     Outside a capture it is the stream's own.  A call that is being captured gets an allocation of its own, from the
     graph's memory, and clears it inside the graph: two graphs never share one, and none holds memory that the cache
     above may give away while the graph lives.
     """
-    if torch.cuda.current_device() != dev.index:
-        with torch.cuda.device(dev):
-            return _call_workspace(dev, params, size_entry)
-    lib = _native.load()
-    nbytes = max(int(getattr(lib, size_entry)(ctypes.byref(params))), 256)
-    stream_ptr = torch.cuda.current_stream(dev).cuda_stream
     if not torch.cuda.is_current_stream_capturing():
         return _workspace(dev, nbytes, stream_ptr)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    rc = lib.rpa_workspace_init(ctypes.c_void_p(ws.data_ptr()), ws.numel(), ctypes.c_void_p(stream_ptr))
+    rc = _native.load().rpa_workspace_init(ctypes.c_void_p(ws.data_ptr()), min(nbytes, _TICKET_BYTES), ctypes.c_void_p(stream_ptr))
     if rc != 0:
         raise RuntimeError(f"rpa_workspace_init failed ({rc}): {_native.last_error()}")
     return ws
