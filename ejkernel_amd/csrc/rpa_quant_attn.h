@@ -33,7 +33,9 @@ struct QuantArgs {
   int tile_tokens;  // tokens of a tile
   int subs;         // tiles side by side for the heads of one token, where they are more than a tile's rows
   int grid;         // workgroups, a multiple of 16
-  uint32_t* tickets;        // [5 * grid], zero between launches: one for each workgroup's cut item of the first stream, four of the second
+  // zero between launches: one for each workgroup's cut item of the first stream, then [level of the tree][workgroup][wavefront]
+  // of the second
+  uint32_t* tickets;
   float* thin_o;            // [2 * grid][16 * D] states of cut items of the first stream, as they lie in registers
   float* thin_ml;           // [2 * grid][16][2]
   float* tile_o;            // [2 * grid][rows * D]
@@ -45,12 +47,13 @@ template <int D, int kParts>
 constexpr int quant_row_tiles() { return kParts == 3 || D == 256 ? 1 : 3; }
 constexpr int kTileStep = 32;
 
+constexpr uint64_t kQuantTicketBytes = 1u << 18;  // of the workspace's head
 constexpr int kThinStep = 128;     // keys a workgroup takes at once in the first stream
 constexpr int kThinPad = 128;      // what an item of the first stream costs beyond its keys, in keys
 constexpr int kTilePad = 64;       // the same of the second
 constexpr int kThinLeast = 256;    // least run of keys per workgroup
 constexpr int kThinWhole = 2048;   // few items of up to so many keys are not cut
-constexpr int kTileLeast = 512;
+constexpr int kTileLeast = 256;
 constexpr float kNoKey = -3.0e38f; // row maximum before any key
 constexpr float kLazy = 8.f;       // the running maximum follows when a logit passes it by 2^8
 constexpr int kAgentScope = 16;    // auxiliary bit of a buffer access: coherent across the device's L2s
@@ -64,10 +67,10 @@ struct Seq {
   int q0, q_len, kv_len;
 };
 
-__device__ __forceinline__ int64_t ramp(int64_t n, int64_t c, int64_t d) {  // sum over i < n of max(0, c + i d)
-  const int64_t i0 = c >= 0 ? 0 : (d - 1 - c) / d;
-  const int64_t m = n > i0 ? n - i0 : 0;
-  return m * (c + i0 * d) + d * (m * (m - 1) / 2);
+__device__ __forceinline__ int64_t ramp(int n, int c, int d) {  // sum over i < n of max(0, c + i d)
+  const int i0 = c >= 0 ? 0 : static_cast<int>(static_cast<uint32_t>(d - 1 - c) / static_cast<uint32_t>(d));
+  const int m = max(n - i0, 0);
+  return static_cast<int64_t>(m) * (c + static_cast<int64_t>(i0) * d) + d * (static_cast<int64_t>(m) * (m - 1) >> 1);
 }
 
 // Keys of the rows of tokens [t0, t1) of a sequence: [first, end).
@@ -87,10 +90,10 @@ __device__ __forceinline__ Range key_range(Args& a, const Seq& q, int t0, int t1
 __device__ __forceinline__ int tiles_of(Args& a, const Seq& q) { return (q.q_len + a.tile_tokens - 1) / a.tile_tokens; }
 // Stream positions in front of tile n (n below the number of tiles), or of all tiles.
 __device__ __forceinline__ int64_t tiles_before(Args& a, const Seq& q, int n, bool all) {
-  const int64_t base = q.kv_len - q.q_len, d = a.tile_tokens;
+  const int base = q.kv_len - q.q_len, d = a.tile_tokens;
   int64_t sum = ramp(n, base + d, d) + static_cast<int64_t>(n) * kTilePad;
-  if (a.p.sliding_window > 0) sum -= ramp(n, base - a.p.sliding_window + 1, d);
-  if (all) sum -= max(base + n * d, static_cast<int64_t>(0)) - max(base + q.q_len, 0);
+  if (a.p.sliding_window > 0) sum -= ramp(n, max(base - a.p.sliding_window + 1, -0x40000000), d);  // (a window beyond every key)
+  if (all) sum -= max(base + n * d, 0) - max(base + q.q_len, 0);
   return sum;
 }
 
@@ -118,10 +121,18 @@ __device__ __forceinline__ Seq load_seq(Args& a, int n, int s) {
 // kFirstTile of kPairUnits, the other the rest.  The workgroups of an XCD hold `block` neighbouring runs, those of the first
 // workgroups in front or, where `back` is set, behind.
 constexpr int kPairUnits = 128, kFirstThin = 76, kFirstTile = 78;
-// 64-bit division where it is needed, 32-bit where that does.
+// x / y of numbers that are not negative: 32 bits nearly always; the rest bit by bit, since the code on the way to the
+// first load is fetched anew by every launch and a 64-bit division is long.
 __device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
   if (static_cast<uint64_t>(x | y) >> 32 == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
-  return x / y;
+  int64_t quotient = 0;
+#pragma unroll 1
+  for (int b = 62; b >= 0; --b) {
+    if ((x >> b) < y) continue;
+    x -= y << b;
+    quotient |= int64_t{1} << b;
+  }
+  return quotient;
 }
 struct Cut {
   int64_t per_unit, rest;  // positions of a unit; the first `rest` units have one more
@@ -707,38 +718,46 @@ __device__ __forceinline__ void tile_item(Args& a, const Seq& q, int s, int hs, 
     const int slots = 2 * a.grid;
     const auto o_rsrc = rsrc_of(a.tile_o, static_cast<uint64_t>(slots) * 64 * kRowTiles * D * 4);
     const int part = self - parts.first;
-    const auto place = [&](int k, int mt, int n) { return (((slot_of(parts, k) * 4 + wave) * kRowTiles + mt) * NO + n) * 1024 + lane * 16; };
-    const auto ml_at = [&](int k, int mt) { return reinterpret_cast<uint64_t*>(a.tile_ml) + (slot_of(parts, k) * 4 + wave) * kRowTiles * 16 + mt * 16 + i; };
+    // The parts meet in a tree, pairs of neighbours first: whoever comes to a node second adds the other's state to its own,
+    // which it still has in registers, and goes on to the next; whoever comes first leaves its state behind.  A wavefront's
+    // rows are its own, so each goes its own way.  A ticket holds the part that waits at its node, plus one.
+    const int wait_part = part + 1;
+    const auto slot_at = [&](int k) { return slot_of(parts, k) * 4 + wave; };
+    const auto place = [&](int k, int mt, int n) { return ((slot_at(k) * kRowTiles + mt) * NO + n) * 1024 + lane * 16; };
+    const auto ml_at = [&](int k, int mt) { return reinterpret_cast<uint64_t*>(a.tile_ml) + (slot_at(k) * kRowTiles + mt) * 16 + i; };
+    int level = 0;
+    for (int span = 1; span < parts.count; span *= 2, ++level) {
+#pragma clang fp contract(off)  // one of the two weights is 1: with both products rounded the sum is the same whoever adds
+      const int node = part & -(2 * span), sibling = (part & span) != 0 ? node : node + span;
+      if (sibling >= parts.count) continue;  // nobody to meet on this level
+      uint32_t* ticket = a.tickets + a.grid + ((level * a.grid + parts.first + node) * 4 + wave);
+      int other = __hip_atomic_load(ticket, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      other = __builtin_amdgcn_readfirstlane(other);
+      if (other == 0) {
 #pragma unroll
-    for (int mt = 0; mt < kRowTiles; ++mt) {
+        for (int mt = 0; mt < kRowTiles; ++mt) {
 #pragma unroll
-      for (int n = 0; n < NO; ++n) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, acc[mt][n]), o_rsrc, place(part, mt, n), 0, kAgentScope);
-      if (g == 0) {
-        const uint64_t both = (static_cast<uint64_t>(__float_as_uint(l[mt])) << 32) | __float_as_uint(m[mt]);
-        __hip_atomic_store(ml_at(part, mt), both, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          for (int n = 0; n < NO; ++n) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, acc[mt][n]), o_rsrc, place(part, mt, n), 0, kAgentScope);
+          if (g == 0) {
+            const uint64_t both = (static_cast<uint64_t>(__float_as_uint(l[mt])) << 32) | __float_as_uint(m[mt]);
+            __hip_atomic_store(ml_at(part, mt), both, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the state is in memory before anybody is told
+        if (lane == 0) other = __hip_atomic_exchange(ticket, static_cast<uint32_t>(wait_part), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        other = __builtin_amdgcn_readfirstlane(other);
+        if (other == 0) return;
       }
-    }
-    // A wavefront's rows are its own: it draws a ticket for them, and the wavefront that draws the last one adds them up.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    uint32_t* ticket = a.tickets + a.grid + 4 * parts.first + wave;
-    uint32_t drawn = 0;
-    if (lane == 0) drawn = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (__builtin_amdgcn_readfirstlane(drawn) + 1 != static_cast<uint32_t>(parts.count)) return;
-    if (lane == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-    for (int mt = 0; mt < kRowTiles; ++mt) {
-      m[mt] = kNoKey, l[mt] = 0.f;
-#pragma unroll
-      for (int n = 0; n < NO; ++n) acc[mt][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
-    for (int k = 0; k < parts.count; ++k) {
+      asm volatile("" ::: "memory");
+      if (lane == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int from = other - 1;
       uint64_t both[kRowTiles];
-      u32x4_t y[kRowTiles][NO];  // all of a part is in flight at once
+      u32x4_t y[kRowTiles][NO];  // all of a state is in flight at once
 #pragma unroll
       for (int mt = 0; mt < kRowTiles; ++mt) {
-        both[mt] = __hip_atomic_load(ml_at(k, mt), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        both[mt] = __hip_atomic_load(ml_at(from, mt), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-        for (int n = 0; n < NO; ++n) y[mt][n] = __builtin_amdgcn_raw_buffer_load_b128(o_rsrc, place(k, mt, n), 0, kAgentScope);
+        for (int n = 0; n < NO; ++n) y[mt][n] = __builtin_amdgcn_raw_buffer_load_b128(o_rsrc, place(from, mt, n), 0, kAgentScope);
       }
 #pragma unroll
       for (int mt = 0; mt < kRowTiles; ++mt) {
@@ -747,7 +766,11 @@ __device__ __forceinline__ void tile_item(Args& a, const Seq& q, int s, int hs, 
         m[mt] = t_new;
         l[mt] = l[mt] * f + lk * fk;
 #pragma unroll
-        for (int n = 0; n < NO; ++n) acc[mt][n] = acc[mt][n] * f + __builtin_bit_cast(f32x4_t, y[mt][n]) * fk;
+        for (int n = 0; n < NO; ++n) {
+          const f32x4_t z = __builtin_bit_cast(f32x4_t, y[mt][n]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[mt][n][e] = acc[mt][n][e] * f + z[e] * fk;
+        }
       }
     }
   }
@@ -814,9 +837,9 @@ __device__ __forceinline__ Run uniform(const Run& r) {
           {uniform(r.first.q0), uniform(r.first.q_len), uniform(r.first.kv_len)}, uniform(r.x), uniform(r.x_end), uniform(r.off)};
 }
 
-// The two streams are functions of their own, so that the registers of one loop are not shared out by the other's.
+
 template <int kCode, int D, typename T, int kParts, bool kCap, bool kWide>
-__device__ __attribute__((noinline)) void thin_phase(uint64_t args) {
+__device__ __forceinline__ void thin_phase(uint64_t args) {
   Args& a = *reinterpret_cast<Args*>(uniform(static_cast<int64_t>(args)));
   Lds<D>& lds = lds_of<D>();
   const Run run = uniform(lds.sched.run[0]);
@@ -844,7 +867,7 @@ __device__ __attribute__((noinline)) void thin_phase(uint64_t args) {
 }
 
 template <int kCode, int D, typename T, int kParts, bool kCap, bool kWide>
-__device__ __attribute__((noinline)) void tile_phase(uint64_t args) {
+__device__ __forceinline__ void tile_phase(uint64_t args) {
   constexpr int kStep = kTileStep;
   Args& a = *reinterpret_cast<Args*>(uniform(static_cast<int64_t>(args)));
   Lds<D>& lds = lds_of<D>();

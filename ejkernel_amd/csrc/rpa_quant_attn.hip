@@ -25,7 +25,7 @@ struct Layout {
 Layout layout(const RpaQuantParams& p, int grid) {
   const uint64_t slots = 2ull * grid, D = padded_dim(p), rows = tile_rows(p);
   Layout l;
-  l.thin_o = kWorkspaceTicketBytes;
+  l.thin_o = kWorkspaceTicketBytes;  // the tickets lie in its first kQuantTicketBytes
   l.thin_ml = l.thin_o + slots * 16 * D * 4;
   l.tile_o = l.thin_ml + slots * 16 * 8;
   l.tile_ml = l.tile_o + slots * rows * D * 4;
@@ -49,6 +49,10 @@ int launch_quant_attention(const RpaQuantParams& p, hipStream_t stream) {
   a.subs = (a.group + rows - 1) / rows;
   if (a.subs > 1) a.tile_tokens = 1;
   a.grid = grid_of();
+  int levels = 0;
+  while ((1 << levels) < a.grid) ++levels;
+  if ((1 + 4ull * levels) * a.grid * sizeof(uint32_t) > kQuantTicketBytes)
+    return fail(RPA_ERR_UNSUPPORTED, "a device of %d compute units: the tickets of its workgroups exceed their place", device_cu_count());
   const Layout l = layout(p, a.grid);
   char* ws = static_cast<char*>(p.workspace);
   a.tickets = reinterpret_cast<uint32_t*>(ws);

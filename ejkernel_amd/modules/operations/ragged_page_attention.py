@@ -156,7 +156,7 @@ def _workspace(device: torch.device, nbytes: int, stream_ptr: int) -> torch.Tens
     return ws
 
 
-_TICKET_BYTES = 1 << 16  # the tickets of the operations that use _call_workspace lie in the first 64 KiB
+_TICKET_BYTES = 1 << 18  # the tickets of the operations that use _call_workspace lie in the first 256 KiB (kQuantTicketBytes)
 
 
 def _call_workspace(dev: torch.device, nbytes: int, stream_ptr: int) -> torch.Tensor:
