@@ -12,7 +12,7 @@ namespace rpa {
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 1024, kFewThreads = 256;
 
 struct Request {
   int q;       // new tokens, negative: ended
@@ -44,6 +44,7 @@ __device__ __forceinline__ int need_of(const RpaBlockTablesParams& p, const Requ
 struct Pair {
   int64_t a, b;
 };
+template <int kWaves>
 __device__ __forceinline__ Pair block_prefix(Pair v, Pair* lds, Pair* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   Pair inc = v;
@@ -52,12 +53,11 @@ __device__ __forceinline__ Pair block_prefix(Pair v, Pair* lds, Pair* total) {
     const int64_t a = __shfl_up(inc.a, o), b = __shfl_up(inc.b, o);
     if (lane >= o) inc.a += a, inc.b += b;
   }
-  __syncthreads();  // lds may still be read from the call before
   if (lane == 63) lds[wave] = inc;
   __syncthreads();
   Pair base = {0, 0}, all = {0, 0};
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) {
+  for (int w = 0; w < kWaves; ++w) {
     const Pair x = lds[w];
     if (w < wave) base.a += x.a, base.b += x.b;
     all.a += x.a, all.b += x.b;
@@ -80,7 +80,8 @@ __device__ __forceinline__ int2 ring_state(const RpaBlockTablesParams& p) {
   return make_int2(head, min(max(p.free_state[1], 0), cap));
 }
 
-__device__ __forceinline__ int ring_place(int64_t i, int cap) { return static_cast<int>(i % cap); }
+// Place i of the ring, i below twice its size.
+__device__ __forceinline__ int ring_place(int64_t i, int cap) { return static_cast<int>(i >= cap ? i - cap : i); }
 
 // Table entries of request s: taken pages behind those it holds, given pages into the ring.  The places written lie
 // behind the ring's free pages, those read among them.
@@ -90,25 +91,35 @@ __device__ __forceinline__ void move_pages(const RpaBlockTablesParams& p, const 
   for (int k = first; k < m.given; k += step) p.free_pages[ring_place(static_cast<int64_t>(m.to) + k, p.num_free_slots)] = row[k];
 }
 
-// Slot and position of flat token t.  `start` are the query starts (n_all + 1 of them).
+// Last s with start[s] <= t of n_all + 1 starts: it holds t where t lies in front of the last of them.
+__device__ __forceinline__ int sequence_of(const int32_t* start, int n_all, int t) {
+  int lo = 0, hi = n_all;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Slot of position pos of request s, which held `have` pages before this step and takes others from place `from` of the
+// ring on.  The page is read where it lay before the step, so it does not matter who has moved already.
+__device__ __forceinline__ int slot_of(const RpaBlockTablesParams& p, int s, int pos, int have, int from) {
+  const int j = pos / p.page_size;
+  const int page = j < have ? p.block_tables[static_cast<size_t>(s) * p.pages_per_seq + j]
+                            : p.free_pages[ring_place(static_cast<int64_t>(from) + (j - have), p.num_free_slots)];
+  return static_cast<int>(static_cast<int64_t>(page) * p.page_size + (pos - j * p.page_size));
+}
+
+// Slot and position of flat token t, from the plan in memory.
 __device__ __forceinline__ void map_token(const RpaBlockTablesParams& p, const int32_t* start, const Move* moves, int n, int t) {
   int slot = -1, pos = -1;
-  const int n_all = p.max_num_seqs;
-  if (t < start[n_all]) {
-    int lo = 0, hi = n_all;  // last s with start[s] <= t: it holds t, since start[s + 1] > t
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (start[mid] <= t) lo = mid;
-      else hi = mid;
-    }
-    const int s = lo;
+  if (t < start[p.max_num_seqs]) {
+    const int s = sequence_of(start, p.max_num_seqs, t);
     if (p.admitted[s]) {
       const Request r = request(p, n, s);
       pos = r.cached + (t - start[s]);
-      const int j = pos / p.page_size;
-      const int page = j < r.have ? p.block_tables[static_cast<size_t>(s) * p.pages_per_seq + j]
-                                  : p.free_pages[ring_place(static_cast<int64_t>(moves[s].from) + (j - r.have), p.num_free_slots)];
-      slot = static_cast<int>(static_cast<int64_t>(page) * p.page_size + (pos - j * p.page_size));
+      slot = slot_of(p, s, pos, r.have, moves[s].from);
     }
   }
   p.slot_mapping[t] = slot;
@@ -117,65 +128,113 @@ __device__ __forceinline__ void map_token(const RpaBlockTablesParams& p, const i
 
 __device__ __forceinline__ int clipped_count(const RpaBlockTablesParams& p) { return min(max(p.num_seqs[0], 0), p.max_num_seqs); }
 
-__global__ __launch_bounds__(kThreads) void block_tables_plan_kernel(RpaBlockTablesParams p, int write_entries) {
-  __shared__ Pair lds[kThreads / 64];
-  const int n_all = p.max_num_seqs, n = clipped_count(p), cap = p.num_free_slots;
-  const int per = (n_all + kThreads - 1) / kThreads;
-  const int s0 = min(static_cast<int64_t>(threadIdx.x) * per, static_cast<int64_t>(n_all)), s1 = min(s0 + per, n_all);
+// What the slots need of the requests, where a thread has one at most.
+template <int kN>
+struct FewLds {
+  int start[kN + 1], cached[kN], from[kN];  // cached: -1 where the request's tokens do not run
+};
+
+template <int kN>
+__global__ __launch_bounds__(kN) void block_tables_plan_kernel(RpaBlockTablesParams p, int write_entries) {
+  constexpr int kWaves = kN / 64;
+  __shared__ Pair lds[3][kWaves];
+  __shared__ FewLds<kN> few;
+  const int n_all = p.max_num_seqs, cap = p.num_free_slots, lane = threadIdx.x & 63;
+  const int per = (n_all + kN - 1) / kN;
+  const int s0 = static_cast<int>(min(static_cast<int64_t>(threadIdx.x) * per, static_cast<int64_t>(n_all))), s1 = min(s0 + per, n_all);
+  const int n = clipped_count(p);
   const int2 ring = ring_state(p);
   Move* moves = reinterpret_cast<Move*>(p.scratch);
+  const Request only = request(p, n, min(s0, n_all - 1));
+  const auto get = [&](int s) { return per == 1 ? only : request(p, n, s); };
 
   Pair sum = {0, 0}, total;
   for (int s = s0; s < s1; ++s) {
-    const Request r = request(p, n, s);
+    const Request r = get(s);
     sum.a += max(r.q, 0);
     sum.b += r.q < 0 ? r.have : 0;
   }
-  const Pair at = block_prefix(sum, lds, &total);  // first token and first page given back of this thread's requests
+  const Pair at = block_prefix<kWaves>(sum, lds[0], &total);  // first token and first page given back of this thread's requests
   sum = {0, 0};
   int64_t end = at.a;
   for (int s = s0; s < s1; ++s) {
-    const Request r = request(p, n, s);
+    const Request r = get(s);
     end += max(r.q, 0);
     sum.a += fits(p, r, end) ? need_of(p, r) : 0;
   }
-  const Pair taken = block_prefix(sum, lds, &total);
-  Pair moved = {0, 0};  // pages taken and given back
+  const Pair taken = block_prefix<kWaves>(sum, lds[1], &total);
+  Pair last = {0, 0};  // behind the last page taken and given back: whoever does not fit, nobody behind it does
   int64_t start = at.a, back = at.b, need = taken.a;
+  Move m = {0, 0, 0, 0};
+  int first_token = 0, cached = -1;
   for (int s = s0; s < s1; ++s) {
-    const Request r = request(p, n, s);
+    const Request r = get(s);
     end = start + max(r.q, 0);
     const bool ok = fits(p, r, end);
     const int want = ok ? need_of(p, r) : 0, gives = r.q < 0 ? r.have : 0;
     const bool in = r.q == 0 || (ok && (want == 0 || need + want <= ring.y));
     const bool out = r.q < 0 && ring.y + back + gives <= cap;  // a ring that cannot hold them: the request stays
-    p.query_start_loc[s] = static_cast<int>(min(start, static_cast<int64_t>(p.total_tokens)));
+    first_token = static_cast<int>(min(start, static_cast<int64_t>(p.total_tokens)));
+    cached = in && r.q > 0 ? r.cached : -1;
+    p.query_start_loc[s] = first_token;
     p.context_lens[s] = in ? r.cached + r.q : 0;
     p.admitted[s] = in ? 1 : 0;
     p.cached_lens_out[s] = s >= n ? p.cached_lens[s] : in ? r.cached + r.q : out ? 0 : r.cached;
-    Move m;
     m.taken = in ? want : 0;
     m.from = ring_place(ring.x + min(need, static_cast<int64_t>(cap)), cap);
     m.given = out ? gives : 0;
     m.to = ring_place(ring.x + ring.y + min(back, static_cast<int64_t>(cap)), cap);
-    moves[s] = m;
-    moved.a += m.taken;
-    moved.b += m.given;
+    if (!write_entries) moves[s] = m;
     start = end;
     need += want;
     back += gives;
+    if (m.taken > 0) last.a = need;
+    if (m.given > 0) last.b = back;
   }
-  block_prefix(moved, lds, &total);
-  if (s0 < n_all && s1 == n_all) p.query_start_loc[n_all] = static_cast<int>(min(start, static_cast<int64_t>(p.total_tokens)));
-  if (threadIdx.x == 0) {
-    p.free_state_out[0] = ring_place(ring.x + total.a, cap);
-    p.free_state_out[1] = static_cast<int>(ring.y - total.a + total.b);
+  const int behind_last = static_cast<int>(min(start, static_cast<int64_t>(p.total_tokens)));
+  if (s0 < n_all && s1 == n_all) p.query_start_loc[n_all] = behind_last;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    last.a = max(last.a, __shfl_xor(last.a, o));
+    last.b = max(last.b, __shfl_xor(last.b, o));
   }
-  if (!write_entries) return;
+  if (lane == 0) lds[2][threadIdx.x >> 6] = last;
+  const int s = threadIdx.x;
+  if (write_entries && s < n_all) {
+    few.start[s] = first_token;
+    few.cached[s] = cached;
+    few.from[s] = m.from;
+    if (s == n_all - 1) few.start[n_all] = behind_last;
+  }
   __syncthreads();
-  const int lane = threadIdx.x & 63;
-  for (int s = threadIdx.x >> 6; s < n; s += kThreads / 64) move_pages(p, moves[s], request(p, n, s).have, s, lane, 64);
-  for (int t = threadIdx.x; t < p.total_tokens; t += kThreads) map_token(p, p.query_start_loc, moves, n, t);
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) last.a = max(last.a, lds[2][w].a), last.b = max(last.b, lds[2][w].b);
+    p.free_state_out[0] = ring_place(ring.x + last.a, cap);
+    p.free_state_out[1] = static_cast<int>(ring.y - last.a + last.b);
+  }
+  if (!write_entries) return;  // else: a thread has one request at most
+  const int have = only.have;
+  // Pages: one for most requests of a decode step, which its thread moves; longer moves by the wavefront, one after another.
+  if (m.taken == 1) p.block_tables[static_cast<size_t>(s) * p.pages_per_seq + have] = p.free_pages[m.from];
+  for (uint64_t long_moves = __ballot(m.taken > 1 || m.given > 0); long_moves != 0; long_moves &= long_moves - 1) {
+    const int l = __ffsll(static_cast<unsigned long long>(long_moves)) - 1;
+    const Move w = {__builtin_amdgcn_readlane(m.taken, l), __builtin_amdgcn_readlane(m.from, l), __builtin_amdgcn_readlane(m.given, l),
+                    __builtin_amdgcn_readlane(m.to, l)};
+    move_pages(p, w, __builtin_amdgcn_readlane(have, l), __builtin_amdgcn_readlane(s, l), lane, 64);
+  }
+  for (int t = threadIdx.x; t < p.total_tokens; t += kN) {
+    int slot = -1, pos = -1;
+    if (t < few.start[n_all]) {
+      const int s = sequence_of(few.start, n_all, t), cached = few.cached[s];
+      if (cached >= 0) {
+        pos = cached + (t - few.start[s]);
+        slot = slot_of(p, s, pos, pages_of(cached, p.page_size), few.from[s]);
+      }
+    }
+    p.slot_mapping[t] = slot;
+    p.positions[t] = pos;
+  }
 }
 
 __global__ __launch_bounds__(256) void block_tables_entries_kernel(RpaBlockTablesParams p, int token_groups) {
@@ -193,8 +252,12 @@ __global__ __launch_bounds__(256) void block_tables_entries_kernel(RpaBlockTable
 }  // namespace
 
 int launch_block_tables(const RpaBlockTablesParams& p, hipStream_t stream) {
+  // The sums take one workgroup: a small one is through its barriers sooner.  It also writes the entries where a thread has
+  // one request and a few tokens.
   const bool few = p.max_num_seqs <= kThreads && p.total_tokens <= 4 * kThreads;
-  hipLaunchKernelGGL(block_tables_plan_kernel, dim3(1), dim3(kThreads), 0, stream, p, few ? 1 : 0);
+  const bool fewer = p.max_num_seqs <= kFewThreads && p.total_tokens <= 4 * kFewThreads;
+  if (fewer) hipLaunchKernelGGL(block_tables_plan_kernel<kFewThreads>, dim3(1), dim3(kFewThreads), 0, stream, p, 1);
+  else hipLaunchKernelGGL(block_tables_plan_kernel<kThreads>, dim3(1), dim3(kThreads), 0, stream, p, few ? 1 : 0);
   if (hipGetLastError() != hipSuccess) return RPA_ERR_LAUNCH;
   if (few) return RPA_OK;
   const int token_groups = (p.total_tokens + 255) / 256, seq_groups = (p.max_num_seqs + 3) / 4;

@@ -3,9 +3,10 @@
 // Update.  For every run of new tokens inside one block and every combined head (K or V of a kv head):
 //   a = max |x| over the run's finite elements,  s = a / 127  or  2^ceil(log2(a / qmax)),  at least the block's old scale
 //   if the run begins inside the block;  code = round(x / s);  if s grew, the codes in front of the run are re-expressed.
-// One wavefront takes one (run, combined head): it reads the rows twice, for the maximum and for the codes (the second
-// time from the caches), and writes one byte per element, so what bounds it is the traffic of the rows, and for single
-// tokens the chain slot -> old scale -> code.  Runs are found from the slots alone: a wavefront looks at 64 tokens at once.
+// One wavefront takes one (run, combined head).  It keeps the rows in registers between the maximum and the codes (runs of
+// more than 64 elements a lane are read twice, the second time from the caches) and writes one byte per element, so what
+// bounds it is the traffic of the rows, and for single tokens the chain slot -> row and old scale -> code.  Runs are found
+// from the slots alone: a wavefront looks at 64 tokens at once.
 #include <algorithm>
 #include <type_traits>
 
@@ -17,23 +18,49 @@ namespace {
 
 constexpr int kPiece = 8;         // elements a lane handles at once
 constexpr int kTokensPerChunk = 64;
+constexpr int kBatch = 8;         // pieces a lane has in flight
 
-// Eight elements from `src` as floats.
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
+
+// Eight elements as they lie in memory, and as floats.
 template <typename T>
-__device__ __forceinline__ void load_piece(const T* __restrict__ src, float (&x)[kPiece]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else {
-    const uint4 w = *reinterpret_cast<const uint4*>(src);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+struct Piece {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* __restrict__ src) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      x[2 * k] = __uint_as_float(u[k] << 16);
-      x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+    for (unsigned k = 0; k < sizeof(T) / 2; ++k) w[k] = reinterpret_cast<const uint4*>(src)[k];
+  }
+  // Largest magnitude so far as an integer, which orders magnitudes as the numbers do, infinity and then NaN on top; bf16 in
+  // both halves of a word at once.
+  __device__ __forceinline__ uint32_t top(uint32_t most) const {
+#pragma unroll
+    for (unsigned k = 0; k < sizeof(T) / 2; ++k) {
+      const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if constexpr (sizeof(T) == 4) most = max(most, u[c] & 0x7fffffffu);
+        else most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, most), __builtin_bit_cast(u16x2_t, u[c] & 0x7fff7fffu)));
+      }
+    }
+    return most;
+  }
+  __device__ __forceinline__ void get(float (&x)[kPiece]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        x[4 * k] = __uint_as_float(w[k].x), x[4 * k + 1] = __uint_as_float(w[k].y);
+        x[4 * k + 2] = __uint_as_float(w[k].z), x[4 * k + 3] = __uint_as_float(w[k].w);
+      }
+    } else {
+      const uint32_t u[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[2 * k] = __uint_as_float(u[k] << 16);
+        x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+      }
     }
   }
-}
+};
 
 // round(x / s) with ties to even, decided on the exact quotient.  `inv` is 1 / s rounded, so x * inv is off by three
 // roundings at most and its nearest integer q by one; r = x - q s is exact in fp32: x and q s are multiples of one unit
@@ -87,6 +114,27 @@ __device__ __forceinline__ uint32_t pack4(const float* x, float s, float inv) {
   }
 }
 
+// The same for finite x of at most code_max * s, without the cases that pack4 looks for.  For int8, adding 1.5 * 2^23 leaves
+// round(x * inv) in the low bits of the sum; `odd` is set where the remainder reaches half a step, which pack4 then decides.
+template <int kCode>
+__device__ __forceinline__ uint32_t pack4_finite(const float* x, float s, float inv, bool& odd) {
+  if constexpr (kCode == kCodeI8) {
+    constexpr float kRound = 12582912.f;
+    uint32_t u[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float y = fmaf(x[k], inv, kRound);
+      odd |= fabsf(fmaf(-(y - kRound), s, x[k])) >= 0.5f * s;
+      u[k] = __float_as_uint(y);
+    }
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[3], u[2], 0x0c0c0400u), __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), 0x05040100u);
+  } else if constexpr (kCode == kCodeE4m3) {
+    return __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, 0, false), true);
+  } else {
+    return __builtin_amdgcn_cvt_pk_bf8_f32(x[2] * inv, x[3] * inv, __builtin_amdgcn_cvt_pk_bf8_f32(x[0] * inv, x[1] * inv, 0, false), true);
+  }
+}
+
 // round(code * old / s): the codes of a word under a larger scale, in fp64, where code * old and q * s are exact products
 // of 32 bits and the quotient is too fine to be mistaken for a middle.  A code that is no number (a cache that somebody
 // else wrote) becomes 0.
@@ -112,6 +160,12 @@ __device__ __forceinline__ uint32_t requantize4(uint32_t w, float old, float s) 
     for (int k = 0; k < 4; ++k) y[k] = off_the_middle(static_cast<double>(code_to_f32<kCode>(w, k)) * old / s);
     return pack4<kCode>(y, 1.f, 1.f);
   }
+}
+
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), o)));
+  return v;
 }
 
 // The scale a run of largest magnitude `a` asks for.
@@ -142,63 +196,119 @@ __global__ __launch_bounds__(256) void quant_update_kernel(RpaQuantUpdateParams 
     if (slot >= pool) slot = -1;
     if (t > 0) before = p.slot_mapping[t - 1];
   }
-  const bool starts = slot >= 0 && (before != slot - 1 || before < 0 || (slot & block_mask) == 0);
-  uint64_t mask = __ballot(starts);
+  const bool follows = slot >= 0 && before >= 0 && before == slot - 1 && (slot & block_mask) != 0;
+  uint64_t mask = __ballot(slot >= 0 && !follows);
+  const uint64_t follow = __ballot(follows);
   const int runs = __popcll(mask), heads = 2 * p.num_kv_heads;
-  const int pieces = p.head_dim / kPiece;
+  const int pieces = p.head_dim / kPiece, step_rows = 64 / pieces, step_pieces = 64 - step_rows * pieces;
+  const int row0 = lane / pieces, piece0 = lane - row0 * pieces;  // this lane's first piece; the next one lies 64 pieces on
   const int workers = gridDim.y * (blockDim.x >> 6);
   int at_run = 0;
   for (int64_t unit = blockIdx.y * (blockDim.x >> 6) + wave; unit < static_cast<int64_t>(runs) * heads; unit += workers) {
-    const int run = static_cast<int>(unit / heads), head = static_cast<int>(unit) - run * heads;
+    const int run = static_cast<int>(unit) / heads, head = static_cast<int>(unit) - run * heads;
     for (; at_run < run; ++at_run) mask &= mask - 1;  // the runs come in order
     const int src_lane = __ffsll(static_cast<unsigned long long>(mask)) - 1;
     const int t0 = blockIdx.x * kTokensPerChunk + src_lane;
     const int s0 = __builtin_amdgcn_readlane(slot, src_lane);
     const int inside = s0 & block_mask;
-    // length of the run: consecutive slots up to the end of the block
-    int n = 1;
-    const int most = min((1 << block_shift) - inside, p.total_tokens - t0);
-    while (n < most) {
-      const int k = n + lane;
-      const bool goes_on = k < most && p.slot_mapping[t0 + k] == s0 + k;
-      const uint64_t b = __ballot(goes_on);
-      const int more = b == ~0ull ? 64 : __ffsll(static_cast<unsigned long long>(~b)) - 1;
-      n += more;
-      if (more < 64) break;
+    // Length of the run: the tokens that follow in this chunk, and if it reaches the chunk's end, those behind it.
+    const uint64_t behind = src_lane == 63 ? 0 : follow >> (src_lane + 1);
+    int n = __ffsll(static_cast<unsigned long long>(~behind));
+    if (src_lane + n == 64) {
+      const int most = min((1 << block_shift) - inside, p.total_tokens - t0);
+      while (n < most) {
+        const int k = n + lane;
+        const uint64_t b = __ballot(k < most && p.slot_mapping[t0 + min(k, most - 1)] == s0 + k);
+        const int more = b == ~0ull ? 64 : __ffsll(static_cast<unsigned long long>(~b)) - 1;
+        n += more;
+        if (more < 64) break;
+      }
     }
     const int j = head >> 1;
     const T* __restrict__ src = (head & 1) ? static_cast<const T*>(p.values) + t0 * p.value_token_stride + j * p.value_head_stride
                                            : static_cast<const T*>(p.keys) + t0 * p.key_token_stride + j * p.key_head_stride;
     const int64_t stride = (head & 1) ? p.value_token_stride : p.key_token_stride;
     const int page = s0 >> page_shift, off = s0 & ((1 << page_shift) - 1);
-    const size_t row0 = ((static_cast<size_t>(page) * heads + head) << page_shift) + off;  // row of the run's first token
+    const size_t first_row = ((static_cast<size_t>(page) * heads + head) << page_shift) + off;
     float* scale = p.kv_scales + ((static_cast<size_t>(page) * heads + head) << (page_shift - block_shift)) + (off >> block_shift);
     const float old = inside > 0 ? *scale : 0.f;
 
-    float a = 0.f;
-    for (int e = lane; e < n * pieces; e += 64) {
-      const int row = e / pieces, piece = e - row * pieces;
-      float x[kPiece];
-      load_piece(src + row * stride + piece * kPiece, x);
+    // Batches of kBatch pieces a lane, all in flight at once; most runs are one batch.
+    const int total = n * pieces;
+    Piece<T> x[kBatch];
+    uint32_t most = 0;
+    int row = row0, piece = piece0;
+    for (int e0 = 0; e0 < total; e0 += 64 * kBatch) {
 #pragma unroll
-      for (int k = 0; k < kPiece; ++k) {
-        const float m = fabsf(x[k]);
-        a = m < INFINITY ? fmaxf(a, m) : a;
+      for (int k = 0; k < kBatch; ++k) {
+        if (e0 + 64 * k >= total) break;
+        const bool real = e0 + 64 * k + lane < total;
+        x[k].load(src + (real ? row * stride + piece * kPiece : 0));
+        row += step_rows, piece += step_pieces;
+        if (piece >= pieces) piece -= pieces, ++row;
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if (e0 + 64 * k >= total) break;
+        most = x[k].top(most);  // a lane behind the last piece holds the first one: it does not change the maximum
       }
     }
-    a = wave_max(a);
+    if constexpr (sizeof(T) == 2) most = max(most & 0xffff0000u, most << 16);
+    most = wave_max_u32(most);
+    const bool finite = most < 0x7f800000u;
+    float a = __uint_as_float(most);
+    if (!finite) {  // seldom: only the finite elements count
+      a = 0.f;
+      row = row0, piece = piece0;
+#pragma unroll 1
+      for (int e = lane; e < total; e += 64) {
+        Piece<T> one;
+        one.load(src + row * stride + piece * kPiece);
+        float y[kPiece];
+        one.get(y);
+#pragma unroll
+        for (int c = 0; c < kPiece; ++c) a = fabsf(y[c]) < INFINITY ? fmaxf(a, fabsf(y[c])) : a;
+        row += step_rows, piece += step_pieces;
+        if (piece >= pieces) piece -= pieces, ++row;
+      }
+      a = wave_max(a);
+    }
     const float want = fresh_scale<kCode>(a);
     const float s = want > old ? want : old > 0.f ? old : want;  // an old scale that is no number counts as none
     const float inv = s > 0.f ? 1.f / s : 0.f;
-    char* dst = static_cast<char*>(p.kv_cache) + row0 * p.head_dim;
-    for (int e = lane; e < n * pieces; e += 64) {
-      const int row = e / pieces, piece = e - row * pieces;
-      float x[kPiece];
-      load_piece(src + row * stride + piece * kPiece, x);
-      uint2 w;
-      w.x = pack4<kCode>(x, s, inv);
-      w.y = pack4<kCode>(x + 4, s, inv);
-      *reinterpret_cast<uint2*>(dst + static_cast<size_t>(e) * kPiece) = w;  // the rows of a block lie together
+    // all elements finite under a scale that the update made itself
+    const bool plain = finite && s > 0.f && (kCode == kCodeI8 || (__float_as_uint(s) & 0x7fffffu) == 0);
+    char* dst = static_cast<char*>(p.kv_cache) + first_row * p.head_dim;
+    row = row0, piece = piece0;
+    for (int e0 = 0; e0 < total; e0 += 64 * kBatch) {
+      if (total > 64 * kBatch) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          if (e0 + 64 * k >= total) break;
+          const bool real = e0 + 64 * k + lane < total;
+          x[k].load(src + (real ? row * stride + piece * kPiece : 0));
+          row += step_rows, piece += step_pieces;
+          if (piece >= pieces) piece -= pieces, ++row;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int e = e0 + 64 * k + lane;
+        if (e0 + 64 * k >= total) break;
+        float y[kPiece];
+        x[k].get(y);
+        uint2 w;
+        bool odd = !plain;
+        if (plain) {
+          w.x = pack4_finite<kCode>(y, s, inv, odd);
+          w.y = pack4_finite<kCode>(y + 4, s, inv, odd);
+        }
+        if (odd) {
+          w.x = pack4<kCode>(y, s, inv);
+          w.y = pack4<kCode>(y + 4, s, inv);
+        }
+        if (e < total) *reinterpret_cast<uint2*>(dst + static_cast<size_t>(e) * kPiece) = w;  // the rows of a block lie together
+      }
     }
     if (inside > 0 && s != old) {
       char* head_rows = dst - static_cast<size_t>(inside) * p.head_dim;
@@ -275,8 +385,8 @@ void by_types(int cache_dtype, int dtype, F&& f) {
 int launch_quant_update(const RpaQuantUpdateParams& p, hipStream_t stream) {
   if (p.total_tokens == 0) return RPA_OK;
   const int chunks = (p.total_tokens + kTokensPerChunk - 1) / kTokensPerChunk;
-  // Enough wavefronts for one (run, head) each where every token is a run of its own (a decode step), and about 4096
-  // workgroups at most where the runs are longer and fewer than the tokens.
+  // Enough wavefronts for one (run, head) each where every token is a run of its own (a decode step), and 4096 workgroups at
+  // most where the runs are longer and fewer than the tokens.
   const int most = (2 * p.num_kv_heads * kTokensPerChunk + 3) / 4;
   const int per_chunk = std::max(1, std::min(most, 4096 / chunks));
   by_types(p.cache_dtype, p.dtype, [&](auto code, auto t) {

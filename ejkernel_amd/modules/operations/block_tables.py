@@ -14,7 +14,7 @@ from typing import NamedTuple
 import torch
 
 from ... import _native
-from .quantized_cache import _call, _on_device
+from .quantized_cache import _call, _check_index_arrays, _on_device
 
 __all__ = ["BlockTables", "BuildBlockTables", "build_block_tables"]
 
@@ -44,15 +44,11 @@ class BuildBlockTables:
         n, pages_per_seq = block_tables.shape
         if not isinstance(num_seqs, torch.Tensor):
             num_seqs = torch.tensor([int(num_seqs)], dtype=torch.int32, device=block_tables.device)
-        for name, t, length in (("query_lens", query_lens, n), ("cached_lens", cached_lens, n), ("free_state", free_state, 2), ("num_seqs", num_seqs, 1)):
-            if t.dim() != 1 or t.shape[0] != length:
-                raise ValueError(f"{name}.shape={tuple(t.shape)} must be ({length},)")
+        _check_index_arrays(("query_lens", query_lens, n), ("cached_lens", cached_lens, n), ("free_state", free_state, 2), ("num_seqs", num_seqs, 1))
         if free_pages.dim() != 1 or free_pages.shape[0] == 0:
             raise ValueError(f"free_pages must be a ring of one page at least, got {tuple(free_pages.shape)}")
-        for name, t in (("query_lens", query_lens), ("cached_lens", cached_lens), ("block_tables", block_tables),
-                        ("free_pages", free_pages), ("free_state", free_state), ("num_seqs", num_seqs)):
-            if t.dtype != torch.int32:
-                raise ValueError(f"{name}.dtype={t.dtype} must be int32")
+        if block_tables.dtype != torch.int32 or free_pages.dtype != torch.int32:
+            raise ValueError(f"block_tables.dtype={block_tables.dtype} and free_pages.dtype={free_pages.dtype} must be int32")
         if not block_tables.is_contiguous() or not free_pages.is_contiguous():
             raise ValueError("block_tables and free_pages must be contiguous: they are updated in place")
         if not 0 < page_size < 2**31:
@@ -66,7 +62,7 @@ class BuildBlockTables:
         # one allocation: the kernels' scratch, at the allocator's alignment, and a view for each result
         sizes = (4 * n + 4, n + 1, n, total_tokens, total_tokens, n, n, 2)
         memory = torch.empty(sum(sizes), dtype=torch.int32, device=block_tables.device)
-        results = memory.split(sizes)[1:]
+        results = torch.unsafe_split_with_sizes(memory, sizes)[1:]  # nothing here is differentiated
         at, places = memory.data_ptr(), []
         for size in sizes:
             places.append(at)

@@ -67,6 +67,15 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     return t, token, head
 
 
+def _check_index_arrays(*arrays: tuple[str, torch.Tensor, int]) -> None:
+    """Name, tensor and length of arrays that are int32 vectors."""
+    for name, t, length in arrays:
+        if t.shape != (length,):
+            raise ValueError(f"{name}.shape={tuple(t.shape)} must be ({length},)")
+        if t.dtype != torch.int32:
+            raise ValueError(f"{name}.dtype={t.dtype} must be int32")
+
+
 def _on_device(op: str, first: torch.Tensor, **others: torch.Tensor) -> int:
     """Index of the device that all of the tensors are on."""
     if not first.is_cuda:
@@ -135,8 +144,8 @@ class QuantizedCacheGather:
         index = _on_device("quantized_cache_gather", kv_cache, kv_scales=kv_scales, slot_mapping=slot_mapping)
         tokens = slot_mapping.shape[0]
         shape = (tokens, heads // 2, head_dim)
-        keys = torch.empty(shape, dtype=dtype, device=kv_cache.device)
-        values = torch.empty(shape, dtype=dtype, device=kv_cache.device)
+        keys = kv_scales.new_empty(shape, dtype=dtype)
+        values = torch.empty_like(keys)
         if tokens == 0:
             return keys, values
         slot_mapping = slot_mapping.contiguous()

@@ -15,7 +15,7 @@ import torch
 
 from ... import _native
 from .configs import QuantizedRaggedPageAttentionConfig
-from .quantized_cache import _VALUE_DTYPES, _call, _check_cache, _current_device, _on_device, _raw_stream, _rows
+from .quantized_cache import _VALUE_DTYPES, _call, _check_cache, _check_index_arrays, _current_device, _on_device, _raw_stream, _rows
 from .ragged_page_attention import _call_workspace, _sinks_per_q_head
 
 __all__ = ["QuantizedRaggedPageAttention", "quantized_ragged_page_attention"]
@@ -50,14 +50,9 @@ class QuantizedRaggedPageAttention:
         max_num_seqs, pages_per_seq = block_tables.shape
         if not isinstance(num_seqs, torch.Tensor):
             num_seqs = torch.tensor([int(num_seqs)], dtype=torch.int32, device=queries.device)
-        for name, t, length in (("context_lens", context_lens, max_num_seqs), ("query_start_loc", query_start_loc, max_num_seqs + 1),
-                                ("num_seqs", num_seqs, 1)):
-            if t.dim() != 1 or t.shape[0] != length:
-                raise ValueError(f"{name}.shape={tuple(t.shape)} must be ({length},)")
-        for name, t in (("context_lens", context_lens), ("block_tables", block_tables), ("query_start_loc", query_start_loc),
-                        ("num_seqs", num_seqs)):
-            if t.dtype != torch.int32:
-                raise ValueError(f"{name}.dtype={t.dtype} must be int32")
+        _check_index_arrays(("context_lens", context_lens, max_num_seqs), ("query_start_loc", query_start_loc, max_num_seqs + 1), ("num_seqs", num_seqs, 1))
+        if block_tables.dtype != torch.int32:
+            raise ValueError(f"block_tables.dtype={block_tables.dtype} must be int32")
         if sliding_window is not None and sliding_window <= 0:
             raise ValueError(f"{sliding_window=} must be positive.")
         if logits_soft_cap is not None and logits_soft_cap == 0.0:
@@ -70,7 +65,7 @@ class QuantizedRaggedPageAttention:
             with torch.cuda.device(index):
                 return self.run(queries, kv_cache, kv_scales, context_lens, block_tables, query_start_loc, num_seqs, softmax_aux,
                                 softmax_scale=softmax_scale, logits_soft_cap=logits_soft_cap, sliding_window=sliding_window, cfg=cfg)
-        out = torch.empty(shape, dtype=queries.dtype, device=queries.device)
+        out = queries.new_empty(shape)
         if total_tokens == 0:
             return out
         queries, token_stride, head_stride = _rows(queries)
