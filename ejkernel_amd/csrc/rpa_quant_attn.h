@@ -196,19 +196,26 @@ __device__ __forceinline__ void split(const float (&x)[8], bf16x8_t (&part)[kPar
   }
 }
 
-// Eight query elements from element d of a row (zeros where the row or the element does not exist).
+// Eight query elements from element d of a row (zeros where the row or the element does not exist), with the sign of the
+// softmax scale.
 template <typename T, int kParts>
-__device__ __forceinline__ void load_q(const T* row, bool real, int d, int head_dim, bf16x8_t (&part)[kParts]) {
+__device__ __forceinline__ void load_q(Args& a, const T* row, bool real, int d, bf16x8_t (&part)[kParts]) {
+  const int head_dim = a.p.head_dim;
+  const uint32_t sign = __float_as_uint(a.p.softmax_scale) & 0x80000000u;
   float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if constexpr (sizeof(T) == 2) {
     u32x4_t w = {0u, 0u, 0u, 0u};
     if (real && d < head_dim) w = *reinterpret_cast<const u32x4_t*>(row + d);
+    w ^= sign | sign >> 16;
     part[0] = __builtin_bit_cast(bf16x8_t, w);
   } else {
     if (real && d < head_dim) {
       const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(row + d), hi = *reinterpret_cast<const f32x4_t*>(row + d + 4);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = lo[e], x[4 + e] = hi[e];
+      for (int e = 0; e < 4; ++e) {
+        x[e] = __uint_as_float(__float_as_uint(lo[e]) ^ sign);
+        x[4 + e] = __uint_as_float(__float_as_uint(hi[e]) ^ sign);
+      }
     }
     split<kParts>(x, part);
   }
@@ -246,23 +253,19 @@ __device__ __forceinline__ void widen_pairs(uint32_t x, uint32_t y, uint32_t (&p
   }
 }
 
-// Loads on either side stay there: they are counted as they come in, so one that the compiler moves behind the others
-// waits for all of them.
 // A lane offset as it stands beside its load, where the load takes it with a scalar base (hoisted, it becomes a pair of
 // registers that is added to the base for every load).
 __device__ __forceinline__ uint32_t here(uint32_t off) {
   asm volatile("" : "+v"(off));
   return off;
 }
+// Loads on either side stay there: they are counted as they come in, so a wait for one that the compiler had moved behind
+// the others would be a wait for all of them.
 __device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
 
 __device__ __forceinline__ f32x4_t mfma(bf16x8_t a, bf16x8_t b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-// Eight logits of a row (keys k0 + 4 g + r and k0 + 16 + 4 g + r of the lane's group g) in units of log2, masked to
-// [lo, hi) where `edge`.
-struct Logits {
-  float x[2][4];
-};
+// A product under its scale: capped in units of log2, or just scaled.
 template <bool kCap>
 __device__ __forceinline__ float scaled(float s, float c, float cap, float inv_cap) {
   if constexpr (kCap) return cap * tanh_fast(s * c * inv_cap);
@@ -436,7 +439,8 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
   };
 
   const float cap = a.p.logits_soft_cap, inv_cap = kCap ? 1.f / cap : 0.f;
-  const float c_scale = kCap ? a.p.softmax_scale : a.p.softmax_scale * kLog2e, cap2 = cap * kLog2e;
+  const float magnitude = fabsf(a.p.softmax_scale);  // its sign is in the queries: logits grow with the products
+  const float c_scale = kCap ? magnitude : magnitude * kLog2e, cap2 = cap * kLog2e;
   // Loads run ahead without a branch, so that every path to a wait has the same loads behind it: the last tile reads itself
   // again (from the caches).
   Pages pg = load_pages(k_begin), pg_next = load_pages(k_begin + stride);
@@ -586,7 +590,7 @@ __device__ __forceinline__ void thin_item(Args& a, const Seq& q, int s, int h, i
   {
     const T* row = static_cast<const T*>(a.p.queries) + (q.q0 + (real ? token : 0)) * a.p.query_token_stride + (real ? head : 0) * a.p.query_head_stride;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) load_q<T, kParts>(row, real, 16 * (g + 4 * (k >> 1)) + 8 * (k & 1), dim, qf[0][k]);
+    for (int k = 0; k < D / 32; ++k) load_q<T, kParts>(a, row, real, 16 * (g + 4 * (k >> 1)) + 8 * (k & 1), qf[0][k]);
   }
   RowState<1, D> st;
   walk<kCode, D, kParts, kCap, kWide, 1>(a, q, s, h, qf, {hi}, range, full_lo, full_hi, base + ka + 32 * wave, base + ((min(kb, keys) + 31) & ~31), 128, st);
@@ -703,7 +707,7 @@ __device__ __forceinline__ void tile_item(Args& a, const Seq& q, int s, int hs, 
     hi[mt] = real ? q_base + row.token + 1 : 0;
     const T* src = static_cast<const T*>(a.p.queries) + (q.q0 + (real ? row.token : 0)) * a.p.query_token_stride + (real ? row.head : 0) * a.p.query_head_stride;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) load_q<T, kParts>(src, real, 16 * (g + 4 * (k >> 1)) + 8 * (k & 1), dim, qf[mt][k]);
+    for (int k = 0; k < D / 32; ++k) load_q<T, kParts>(a, src, real, 16 * (g + 4 * (k >> 1)) + 8 * (k & 1), qf[mt][k]);
   }
   const int full_lo = a.p.sliding_window > 0 ? max(q_base + t1 - a.p.sliding_window, 0) : 0;  // keys every row sees
   const int full_hi = q_base + t0 + 1;
@@ -816,9 +820,7 @@ struct SchedLds {
 
 template <int D>
 struct Lds {
-  union {
-    ThinLds<D> thin;
-  };
+  ThinLds<D> thin;
   SchedLds sched;
 };
 template <int D>

@@ -40,6 +40,7 @@ uint64_t quant_attention_workspace(const RpaQuantParams& p) { return layout(p, g
 int launch_quant_attention(const RpaQuantParams& p, hipStream_t stream) {
   QuantArgs a;
   a.p = p;
+  a.p.sliding_window = std::min(p.sliding_window, 1 << 30);  // no sequence has more keys, and positions minus a window stay in 32 bits
   a.page_shift = __builtin_ctz(p.page_size);
   a.block_shift = __builtin_ctz(p.scale_block);
   a.group = p.num_q_heads / p.num_kv_heads;

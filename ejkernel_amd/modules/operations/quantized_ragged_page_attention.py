@@ -138,7 +138,8 @@ def quantized_ragged_page_attention(
             views with strides of whole 16-byte pieces are read in place.
         kv_cache: ``[num_pages, 2 * num_kv_heads, page_size, head_dim]`` int8, float8_e4m3fn or float8_e5m2;
             K of kv head ``j`` at ``2j``, V at ``2j + 1``.  Every value a sequence can see must be finite.
-        kv_scales: ``[num_pages, 2 * num_kv_heads, page_size // block]`` float32.
+        kv_scales: ``[num_pages, 2 * num_kv_heads, page_size // block]`` float32, finite and not negative where a
+            sequence can see the block.
         context_lens: ``[max_num_seqs]`` int32, keys of each sequence including its query tokens.
         block_tables: ``[max_num_seqs, pages_per_seq]`` int32; entries behind a sequence's pages are not read.
         query_start_loc: ``[max_num_seqs + 1]`` int32 cumulative query lengths.

@@ -286,11 +286,11 @@ int rpa_ragged_decode_launch(const RpaRaggedDecodeParams* params, void* hip_stre
  *
  *   kv_cache  [num_pages, 2*num_kv_heads, page_size, head_dim] codes, int8 / e4m3 / e5m2; K of kv head j at 2j, V at
  *             2j + 1.  The tokens of a page lie together for each head, so the block one scale covers is contiguous.
- *   kv_scales [num_pages, 2*num_kv_heads, page_size / scale_block] fp32; element = code * scale of its block.
+ *   kv_scales [num_pages, 2*num_kv_heads, page_size / scale_block] fp32, not negative; element = code * scale of its block.
  *
  * head_dim is a multiple of 16 from 16 to 256, page_size a power of two from 4 to 32768, scale_block a power of two from 4
- * to page_size, num_pages * page_size below 2^31, a page
- * smaller than 2^31 bytes, pages_per_seq * page_size at most 2^30.  Slot = page * page_size + offset names a token's place in the pool.
+ * to page_size, num_pages * page_size below 2^31, a page smaller than 2^31 bytes, pages_per_seq * page_size at most 2^30.
+ * Slot = page * page_size + offset names a token's place in the pool.
  */
 
 /* Attention over that cache: queries of every sequence against its keys, causal from the end of its context, with the

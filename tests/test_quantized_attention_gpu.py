@@ -74,6 +74,25 @@ def test_negative_and_zero_scale():
         run(Batch([(1, 100), (40, 50)], q_heads=4, kv_heads=2, dim=64, page=16, block=16, kind="int8", scale=scale, seed=1))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_negative_scale_of_large_logits(dtype):
+    """Logits of thousands of either sign: the running maximum has to follow the scaled ones, not the products."""
+    run(Batch([(1, 300), (3, 90), (70, 150)], q_heads=4, kv_heads=2, dim=64, page=16, block=16, kind="int8", dtype=dtype, scale=-40.0, seed=3))
+    run(Batch([(1, 300), (70, 150)], q_heads=4, kv_heads=2, dim=64, page=8, block=8, kind="e4m3", dtype=dtype, scale=-40.0, cap=900.0, seed=4))
+
+
+def test_largest_window_is_no_window():
+    """Requests that have more tokens than keys, too: their first rows lie in front of every key."""
+    b = Batch([(1, 70), (60, 100), (33, 33)], q_heads=4, kv_heads=2, dim=64, page=16, block=16, kind="int8", seed=6)
+    want = run(b)
+    assert torch.equal(quantized_ragged_page_attention(*b.args(), softmax_scale=b.scale, sliding_window=2**31 - 1), want)
+    lens = b.args()[3] // 2  # the pages stay whose keys these are
+    args = [*b.args()[:3], lens, *b.args()[4:]]
+    want = quantized_ragged_page_attention(*args)
+    assert torch.isfinite(want).all()
+    assert torch.equal(quantized_ragged_page_attention(*args, sliding_window=2**31 - 1), want)
+
+
 def test_extreme_logits_and_scales():
     """Logits of thousands, scales next to the least and the largest that an update makes, blocks of zeros."""
     b = Batch([(1, 200), (50, 120)], q_heads=4, kv_heads=2, dim=64, page=16, block=16, kind="e4m3", dtype="fp32", seed=2, scale=20.0)
