@@ -183,6 +183,90 @@ __device__ __forceinline__ float fresh_scale(float a) {
   }
 }
 
+// The scale of rows that were given: at least the block's old one (one that is no number counts as none).
+template <int kCode>
+__device__ __forceinline__ float next_scale(float a, float old) {
+  const float want = fresh_scale<kCode>(a);
+  return want > old ? want : old > 0.f ? old : want;
+}
+
+// Codes of a piece; `plain`: all of its elements are finite, under a scale that an update made.
+template <int kCode, typename T>
+__device__ __forceinline__ uint2 codes_of(const Piece<T>& x, float s, float inv, bool plain) {
+  float y[kPiece];
+  x.get(y);
+  uint2 w = {0u, 0u};
+  bool odd = !plain;
+  if (plain) {
+    w.x = pack4_finite<kCode>(y, s, inv, odd);
+    w.y = pack4_finite<kCode>(y + 4, s, inv, odd);
+  }
+  if (odd) {
+    w.x = pack4<kCode>(y, s, inv);
+    w.y = pack4<kCode>(y + 4, s, inv);
+  }
+  return w;
+}
+template <int kCode>
+__device__ __forceinline__ bool is_plain(bool finite, float s) {
+  return finite && s > 0.f && (kCode == kCodeI8 || (__float_as_uint(s) & 0x7fffffu) == 0);
+}
+
+// Re-expresses the pieces lane, lane + lanes, ... < n in front of `rows` under a scale that has grown.
+template <int kCode>
+__device__ __forceinline__ void requantize(char* rows, int n, int lane, int lanes, float old, float s) {
+  const float was = old > 0.f ? old : 0.f;
+  for (int e = lane; e < n; e += lanes) {
+    uint2* at = reinterpret_cast<uint2*>(rows + static_cast<size_t>(e) * kPiece);
+    uint2 w = *at;
+    w.x = requantize4<kCode>(w.x, was, s);
+    w.y = requantize4<kCode>(w.y, was, s);
+    *at = w;
+  }
+}
+
+// 64 tokens of which no two are neighbours in a block (a decode step): a row of head_dim elements fills only a part of a
+// wavefront, so that 64 / lanes rows are taken at once, `lanes` being the power of two that holds one.
+template <int kCode, typename T>
+__device__ __forceinline__ void update_single_rows(const RpaQuantUpdateParams& p, int page_shift, int block_shift, int slot, int worker, int workers) {
+  const int lane = threadIdx.x & 63, heads = 2 * p.num_kv_heads, pieces = p.head_dim / kPiece, lane_bits = 32 - __clz(pieces - 1), lanes = 1 << lane_bits;
+  const int piece = lane & (lanes - 1), units = min(kTokensPerChunk, p.total_tokens - static_cast<int>(blockIdx.x) * kTokensPerChunk) * heads;
+  for (int unit0 = worker << (6 - lane_bits); unit0 < units; unit0 += workers << (6 - lane_bits)) {
+    const int unit = min(unit0 + (lane >> lane_bits), units - 1), token = unit / heads, head = unit - token * heads, j = head >> 1;
+    const int s0 = __shfl(slot, token);
+    const bool real = s0 >= 0 && unit0 + (lane >> lane_bits) < units;
+    const int page = real ? s0 >> page_shift : 0, off = s0 & ((1 << page_shift) - 1), inside = s0 & ((1 << block_shift) - 1);
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * kTokensPerChunk + token;
+    const T* src = (head & 1) ? static_cast<const T*>(p.values) + t * p.value_token_stride + j * p.value_head_stride
+                              : static_cast<const T*>(p.keys) + t * p.key_token_stride + j * p.key_head_stride;
+    const size_t line = static_cast<size_t>(page) * heads + head;
+    float* scale = p.kv_scales + (line << (page_shift - block_shift)) + (off >> block_shift);
+    const float old = real && inside > 0 ? *scale : 0.f;
+    Piece<T> x;
+    x.load(src + (piece < pieces ? piece * kPiece : 0));  // lanes behind the row hold its first piece: no change to the maximum
+    uint32_t most = x.top(0u);
+    if constexpr (sizeof(T) == 2) most = max(most & 0xffff0000u, most << 16);
+    uint32_t row_most = most;
+    for (int o = lanes >> 1; o > 0; o >>= 1) row_most = max(row_most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(row_most), o)));
+    const bool finite = row_most < 0x7f800000u;
+    float a = __uint_as_float(row_most);
+    if (__any(!finite)) {  // seldom: only the finite elements count
+      float y[kPiece], b = 0.f;
+      x.get(y);
+#pragma unroll
+      for (int c = 0; c < kPiece; ++c) b = fabsf(y[c]) < INFINITY ? fmaxf(b, fabsf(y[c])) : b;
+      for (int o = lanes >> 1; o > 0; o >>= 1) b = fmaxf(b, __shfl_xor(b, o));
+      a = b;
+    }
+    const float s = next_scale<kCode>(a, old), inv = s > 0.f ? 1.f / s : 0.f;
+    if (!real) continue;
+    char* dst = static_cast<char*>(p.kv_cache) + ((line << page_shift) + off) * p.head_dim;
+    if (piece < pieces) *reinterpret_cast<uint2*>(dst + piece * kPiece) = codes_of<kCode>(x, s, inv, is_plain<kCode>(finite, s));
+    if (inside > 0 && s != old) requantize<kCode>(dst - static_cast<size_t>(inside) * p.head_dim, inside * pieces, piece, lanes, old, s);
+    if (piece == 0 && (inside == 0 || s != old)) *scale = s;
+  }
+}
+
 template <int kCode, typename T>
 __global__ __launch_bounds__(256) void quant_update_kernel(RpaQuantUpdateParams p, int page_shift, int block_shift) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -202,9 +286,17 @@ __global__ __launch_bounds__(256) void quant_update_kernel(RpaQuantUpdateParams 
   const int runs = __popcll(mask), heads = 2 * p.num_kv_heads;
   const int pieces = p.head_dim / kPiece, step_rows = 64 / pieces, step_pieces = 64 - step_rows * pieces;
   const int row0 = lane / pieces, piece0 = lane - row0 * pieces;  // this lane's first piece; the next one lies 64 pieces on
-  const int workers = gridDim.y * (blockDim.x >> 6);
+  const int worker = blockIdx.y * (blockDim.x >> 6) + wave, workers = gridDim.y * (blockDim.x >> 6);
+  const int behind_chunk = (blockIdx.x + 1) * kTokensPerChunk;
+  if (follow == 0) {
+    const int last = __builtin_amdgcn_readlane(slot, 63);
+    if (last < 0 || behind_chunk >= p.total_tokens || p.slot_mapping[behind_chunk] != last + 1 || ((last + 1) & block_mask) == 0) {
+      update_single_rows<kCode, T>(p, page_shift, block_shift, slot, worker, workers);
+      return;
+    }
+  }
   int at_run = 0;
-  for (int64_t unit = blockIdx.y * (blockDim.x >> 6) + wave; unit < static_cast<int64_t>(runs) * heads; unit += workers) {
+  for (int64_t unit = worker; unit < static_cast<int64_t>(runs) * heads; unit += workers) {
     const int run = static_cast<int>(unit) / heads, head = static_cast<int>(unit) - run * heads;
     for (; at_run < run; ++at_run) mask &= mask - 1;  // the runs come in order
     const int src_lane = __ffsll(static_cast<unsigned long long>(mask)) - 1;
@@ -273,11 +365,8 @@ __global__ __launch_bounds__(256) void quant_update_kernel(RpaQuantUpdateParams 
       }
       a = wave_max(a);
     }
-    const float want = fresh_scale<kCode>(a);
-    const float s = want > old ? want : old > 0.f ? old : want;  // an old scale that is no number counts as none
-    const float inv = s > 0.f ? 1.f / s : 0.f;
-    // all elements finite under a scale that the update made itself
-    const bool plain = finite && s > 0.f && (kCode == kCodeI8 || (__float_as_uint(s) & 0x7fffffu) == 0);
+    const float s = next_scale<kCode>(a, old), inv = s > 0.f ? 1.f / s : 0.f;
+    const bool plain = is_plain<kCode>(finite, s);
     char* dst = static_cast<char*>(p.kv_cache) + first_row * p.head_dim;
     row = row0, piece = piece0;
     for (int e0 = 0; e0 < total; e0 += 64 * kBatch) {
@@ -295,31 +384,11 @@ __global__ __launch_bounds__(256) void quant_update_kernel(RpaQuantUpdateParams 
       for (int k = 0; k < kBatch; ++k) {
         const int e = e0 + 64 * k + lane;
         if (e0 + 64 * k >= total) break;
-        float y[kPiece];
-        x[k].get(y);
-        uint2 w;
-        bool odd = !plain;
-        if (plain) {
-          w.x = pack4_finite<kCode>(y, s, inv, odd);
-          w.y = pack4_finite<kCode>(y + 4, s, inv, odd);
-        }
-        if (odd) {
-          w.x = pack4<kCode>(y, s, inv);
-          w.y = pack4<kCode>(y + 4, s, inv);
-        }
+        const uint2 w = codes_of<kCode>(x[k], s, inv, plain);
         if (e < total) *reinterpret_cast<uint2*>(dst + static_cast<size_t>(e) * kPiece) = w;  // the rows of a block lie together
       }
     }
-    if (inside > 0 && s != old) {
-      char* head_rows = dst - static_cast<size_t>(inside) * p.head_dim;
-      const float was = old > 0.f ? old : 0.f;
-      for (int e = lane; e < inside * pieces; e += 64) {
-        uint2 w = *reinterpret_cast<const uint2*>(head_rows + static_cast<size_t>(e) * kPiece);
-        w.x = requantize4<kCode>(w.x, was, s);
-        w.y = requantize4<kCode>(w.y, was, s);
-        *reinterpret_cast<uint2*>(head_rows + static_cast<size_t>(e) * kPiece) = w;
-      }
-    }
+    if (inside > 0 && s != old) requantize<kCode>(dst - static_cast<size_t>(inside) * p.head_dim, inside * pieces, lane, 64, old, s);
     if (lane == 0 && (inside == 0 || s != old)) *scale = s;
   }
 }
@@ -385,9 +454,11 @@ void by_types(int cache_dtype, int dtype, F&& f) {
 int launch_quant_update(const RpaQuantUpdateParams& p, hipStream_t stream) {
   if (p.total_tokens == 0) return RPA_OK;
   const int chunks = (p.total_tokens + kTokensPerChunk - 1) / kTokensPerChunk;
-  // Enough wavefronts for one (run, head) each where every token is a run of its own (a decode step), and 4096 workgroups at
-  // most where the runs are longer and fewer than the tokens.
-  const int most = (2 * p.num_kv_heads * kTokensPerChunk + 3) / 4;
+  // Enough lanes for all rows of a chunk at once where every token is a run of its own (a decode step), and 4096 workgroups
+  // at most where the runs are longer and fewer than the tokens.
+  int lanes = 1;
+  while (lanes * kPiece < p.head_dim) lanes *= 2;
+  const int most = (2 * p.num_kv_heads * kTokensPerChunk * lanes + 255) / 256;
   const int per_chunk = std::max(1, std::min(most, 4096 / chunks));
   by_types(p.cache_dtype, p.dtype, [&](auto code, auto t) {
     hipLaunchKernelGGL((quant_update_kernel<decltype(code)::value, decltype(t)>), dim3(chunks, per_chunk), dim3(256), 0, stream, p,
