@@ -9,15 +9,29 @@
 //
 // One launch of 2 workgroups per compute unit.  The batch is two streams of keys.  A sequence with at most 16 query rows
 // per kv head (a decode step) is one item per kv head of the first stream: its rows fill one 16-wide matrix tile, and the
-// four wavefronts of a workgroup take every fourth tile of 32 keys and meet in LDS at its end; nothing is shared between
-// them on the way, so they load straight into registers.  What bounds this stream is memory.  Other sequences are cut into
-// tiles of rows, an item each of the second stream: the workgroup widens 8 KiB of K and of V codes at a time into LDS, in
-// the order in which the matrix unit takes them, and each wavefront multiplies them with its own rows.  What bounds it is
-// matrix, LDS and exp throughput.  Each stream is cut into equal runs of keys, one per workgroup, wherever the cut falls:
-// few long sequences, one long chunk and a ragged batch all fill the device.  An item that is cut leaves its parts'
-// (maximum, sum, output) in the workspace, and the workgroup that hands in the last part adds them up in stream order,
-// so that results do not depend on who that is.  Half of the workgroups take their run of the second stream first, so that
-// one workgroup of a compute unit waits for memory while the other multiplies.
+// four wavefronts of a workgroup take every fourth tile of 32 keys and meet in LDS at its end.  Other sequences are cut into
+// tiles of rows, an item each of the second stream: each wavefront has rows of its own (quant_row_tiles times 16) and walks
+// all of the item's keys.  In both a wavefront loads K and V straight into the registers that the matrix unit takes them
+// from, so nothing waits for another wavefront on the way (with the tiles' codes widened through LDS, the workgroup in
+// step, 16 chunks of 512 tokens after 4096 took 410 us; so, 295 to 320 us).
+//
+// Each stream is cut into equal runs of keys, one per workgroup, wherever the cut falls: few long sequences, one long chunk
+// and a ragged batch all fill the device.  Parts of an item that is cut meet through the workspace: those of the first
+// stream are added up by the workgroup that hands in the last one, in stream order, those of the second in a binary tree.
+// Either way the result does not depend on who comes last.  Half of the workgroups take their run of the second stream
+// first, so that one workgroup of a compute unit waits for memory while the other multiplies.
+//
+// What bounds it, on a device that copies at 4.9 TB/s, reads at 6.2 TB/s and multiplies bf16 matrices at 1325 TFLOP/s:
+//   - decode, 256 sequences of up to 8192 keys, 32/8 heads of 128: the reads, 2.3 GB in 423 us = 5.5 TB/s;
+//   - decode behind a window of 4096 (64 x 4 tokens, 16/8 heads of 256): the reads, 172 us = 4.9 TB/s;
+//   - chunks: instruction issue.  A 32-key step of a 48-row wavefront at head_dim 128 is 48 matrix instructions of 16
+//     cycles and about 330 vector instructions -- 80 to widen the codes (e4m3; 210 for int8), 67 for each 16 rows' softmax,
+//     24 of them exponentials of four times the cost -- so that the vector units are busy 78 % of the time and the matrix
+//     units 33 %: 725 TFLOP/s (e4m3) and 670 (int8) for 16 chunks of 512 tokens, 775 for 2 x 8192 tokens;
+//   - fp32 queries: the same with three products for one and the splitting of probabilities on top: 122 TFLOP/s of plain
+//     products for a mixed batch at head_dim 96, which runs as 128;
+//   - few short sequences: the chain of dependent loads in front of the first product (lengths, their sums, page, codes),
+//     12 us for 8 sequences of up to 1024 keys.
 #pragma once
 
 #include "rpa_quant.h"
@@ -38,11 +52,13 @@ struct QuantArgs {
   uint32_t* tickets;
   float* thin_o;            // [2 * grid][16 * D] states of cut items of the first stream, as they lie in registers
   float* thin_ml;           // [2 * grid][16][2]
-  float* tile_o;            // [2 * grid][rows * D]
+  float* tile_o;            // [2 * grid][rows * D], the same of the second
   float* tile_ml;           // [2 * grid][rows][2]
 };
 
-// Shape of the second stream's tiles for a (padded) head_dim: keys per step, and 16-row tiles per wavefront.
+// The second stream's tiles for a (padded) head_dim: 16-row tiles per wavefront, and keys per step.  Three share the
+// widening of a key among 48 rows in what registers there are at two workgroups per compute unit; head_dim 256 has room for
+// one, and so have fp32 queries (two spill: 113 in place of 104 us for a mixed batch at head_dim 96).
 template <int D, int kParts>
 constexpr int quant_row_tiles() { return kParts == 3 || D == 256 ? 1 : 3; }
 constexpr int kTileStep = 32;
@@ -52,7 +68,8 @@ constexpr int kThinStep = 128;     // keys a workgroup takes at once in the firs
 constexpr int kThinPad = 128;      // what an item of the first stream costs beyond its keys, in keys
 constexpr int kTilePad = 64;       // the same of the second
 constexpr int kThinLeast = 256;    // least run of keys per workgroup
-constexpr int kThinWhole = 2048;   // few items of up to so many keys are not cut
+constexpr int kThinUneven = 1024;  // what cuts at any place cost over cuts into equal parts, in keys of a run
+constexpr int kThinMeet = 384;     // what a cut costs at all
 constexpr int kTileLeast = 256;
 constexpr float kNoKey = -3.0e38f; // row maximum before any key
 constexpr float kLazy = 8.f;       // the running maximum follows when a logit passes it by 2^8
@@ -118,7 +135,8 @@ __device__ __forceinline__ Seq load_seq(Args& a, int n, int s) {
 // A cut of a stream of `total` positions over `n` workgroups: run w is [bound(w), bound(w + 1)).  Where the whole grid takes
 // part, two workgroups share a compute unit, and the one that was there first gets the larger part of its issue slots and
 // of its memory requests: with equal runs it ends at three quarters of the other's time.  So it gets the longer run: kFirstThin or
-// kFirstTile of kPairUnits, the other the rest.  The workgroups of an XCD hold `block` neighbouring runs, those of the first
+// kFirstTile of kPairUnits, the other the rest (2 x 8192 tokens: 865 us at 64, 816 at 76, 800 at 80; 16 chunks of 512 after
+// 4096: 304, 319 and 335; decode steps are alike from 72 to 88).  The workgroups of an XCD hold `block` neighbouring runs, those of the first
 // workgroups in front or, where `back` is set, behind.
 constexpr int kPairUnits = 128, kFirstThin = 76, kFirstTile = 78;
 // x / y of numbers that are not negative: 32 bits nearly always; the rest bit by bit, since the code on the way to the
@@ -806,7 +824,7 @@ __device__ __forceinline__ int place_in_cut(int b, int n) {
 struct Run {
   Cut cut;
   int self, seq, n;
-  int fixed;  // first stream: positions of every item, 0 where they are its keys and kThinPad
+  int fixed;  // first stream: positions of every item (a multiple of the run), 0 where they are its keys and kThinPad
   Seq first;  // lengths of sequence `seq`
   int64_t x, x_end, off;
 };
@@ -915,7 +933,7 @@ __global__ __launch_bounds__(256, 2) void quant_attention_kernel(QuantArgs) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n = min(max(a.p.num_seqs[0], 0), a.p.max_num_seqs);
 
-  // Lengths of the two streams; of the first also the longest item and how many there are.
+  // Lengths of the two streams; of the first also the longest item and how many sequences there are.
   const int per = (a.p.max_num_seqs + 255) >> 8;
   const int s0 = min(static_cast<int>(threadIdx.x) * per, a.p.max_num_seqs), s1 = min(s0 + per, a.p.max_num_seqs);
   auto length = [&](const Seq& q, bool thin) {
@@ -956,9 +974,21 @@ __global__ __launch_bounds__(256, 2) void quant_attention_kernel(QuantArgs) {
     seqs_all += sched.seqs[w];
     longest = max(longest, sched.longest[w]);
   }
-  // Few short items: a workgroup each, so that none is cut and no state goes through memory.
+  // Few items: as many equal parts for each as there are workgroups, one for a compute unit, and places for the longest.  A
+  // run that holds the end of an item and the start of the next takes 6 us longer, in which a workgroup walks kThinUneven
+  // keys, so items of different lengths get places of their own unless the longest is that much longer than an even run
+  // (8 x 8192 keys of 8 heads: 39 us cut anywhere, 34 us in equal parts; 24 x 1024: 27 and 20 us); and parts that meet
+  // take 2 us, kThinMeet keys, so short items are not cut (8 x 512 keys: 15.2 us in two parts, 14.7 us in one; 8 x 1024:
+  // 15.8 us in four, 18.8 us in one).
   const int64_t items = static_cast<int64_t>(seqs_all) * a.p.num_kv_heads;
-  const int fixed = items <= a.grid / 2 && longest <= kThinWhole ? longest + kThinPad : 0;
+  int parts = 0, piece = 0;
+  if (items > 0 && items <= a.grid / 2) {
+    parts = max(min(a.grid / 2 / static_cast<int>(items), longest / kThinLeast), 1);
+    if (longest - longest / parts < kThinMeet) parts = 1;
+    piece = max(((longest - 1) / parts + kThinStep) & -kThinStep, kThinStep);  // parts * piece >= longest
+    if (piece > total[0] / (a.grid / 2) + kThinUneven) parts = 0;
+  }
+  const int fixed = parts * piece;
   if (fixed > 0) {
     sum[0] = static_cast<int64_t>(seqs) * a.p.num_kv_heads * fixed;
     before[0] = static_cast<int64_t>(seqs_before) * a.p.num_kv_heads * fixed;
@@ -972,7 +1002,7 @@ __global__ __launch_bounds__(256, 2) void quant_attention_kernel(QuantArgs) {
     r.fixed = c == 0 ? fixed : 0;
     const int64_t most = max(total[c] / (c == 0 ? kThinLeast : kTileLeast), static_cast<int64_t>(1));  // workgroups worth their while
     const bool whole = most >= a.grid && r.fixed == 0;
-    r.cut.n = whole ? a.grid : static_cast<int>(r.fixed > 0 ? items : min(most, static_cast<int64_t>(a.grid / 2)));
+    r.cut.n = whole ? a.grid : static_cast<int>(r.fixed > 0 ? items * parts : min(most, static_cast<int64_t>(a.grid / 2)));
     r.cut.block = whole ? a.grid / 8 : 2 * r.cut.n;
     r.cut.pair = whole ? kPairUnits : 2;
     r.cut.lead = !whole ? 1 : c == 0 ? kFirstThin : kPairUnits - kFirstTile;
