@@ -75,14 +75,14 @@ __device__ __forceinline__ float round_quotient(float x, float s, float inv) {
   return q;
 }
 
-// A quotient in fp64 as the fp32 number that an 8-bit floating type rounds alike: where the conversion is not exact the
-// number is moved off the middle between two codes, to the side the quotient lies on.  (Quotients of 32-bit products lie
-// on a middle or further from it than fp64 rounds.)
+// A quotient in fp64 as an fp32 number that an 8-bit floating type rounds alike: cut off towards zero, with the last bit set
+// where that is not exact.  Such a number lies on the quotient's side of every middle between two codes, whose last bit is
+// clear.  (Quotients of 32-bit products lie on a middle or further from it than fp64 rounds.)
 __device__ __forceinline__ float off_the_middle(double v) {
   const float f = static_cast<float>(v);
   const double d = static_cast<double>(f);
   if (d == v) return f;
-  return __uint_as_float(__float_as_uint(f) + (fabs(d) < fabs(v) ? 1u : ~0u));
+  return __uint_as_float((__float_as_uint(f) - (fabs(d) > fabs(v) ? 1u : 0u)) | 1u);
 }
 
 // Code of x under scale s (0 where the block is all zeros).  Infinities saturate, NaN is 0.  Where the scale of a floating

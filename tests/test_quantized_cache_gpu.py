@@ -185,3 +185,51 @@ def test_update_in_a_graph_follows_its_slots():
         np.testing.assert_array_equal(sc.cpu().numpy(), scales)
         wk, _ = oracle.cache_gather(codes, scales, s, "int8")
         assert torch.equal(back[0].cpu(), torch.from_numpy(wk.astype(np.float32)).to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,dim", [(1, 16), (3, 48), (2, 128), (2, 256)])
+def test_single_tokens_beside_runs(heads, dim, kind):
+    """Single tokens alone, with holes, and in front of a run that begins at the last token of 64 or goes on behind them."""
+    rng = np.random.default_rng(dim)
+    page, block = 32, 8
+    single = lambda n, first: [(first + i) * page + int(rng.integers(0, page)) for i in range(n)]  # noqa: E731
+    for slots in (single(64, 0), single(130, 0), single(40, 0) + [-1] * 30 + single(9, 40), single(63, 0) + [70 * page + 3 + i for i in range(12)],
+                  single(63, 0) + [70 * page + 7, 70 * page + 8] + single(5, 90), single(64, 0) + [80 * page + i for i in range(70)],
+                  [5 * page + 30 + i for i in range(2)] + [6 * page], [-1] * 64 + single(3, 0), [9 * page + 31]):
+        codes, scales = random_cache(rng, 150, 2 * heads, page, dim, block, kind)
+        keys, values = rows(rng, len(slots), heads, dim, "bf16"), rows(rng, len(slots), heads, dim, "bf16")
+        keys[:: 7, :, 1::2] = float("inf")
+        values[2:: 9, 0, 0] = float("nan")
+        check_update(keys, values, codes, scales, slots, kind)
+
+
+def test_a_pool_beyond_four_gigabytes():
+    """Codes and scales beyond 2**32 bytes: the same rows as in a small pool, written, read and attended to."""
+    from ejkernel_amd.modules import quantized_ragged_page_attention
+
+    rng = np.random.default_rng(1)
+    heads, dim, page, block, lengths = 8, 128, 16, 4, [100, 37]
+    need = sum(-(-n // page) for n in lengths)
+    keys, values = rows(rng, sum(lengths), heads, dim, "bf16", 0.5).to("cuda:0"), rows(rng, sum(lengths), heads, dim, "bf16", 0.5).to("cuda:0")
+    queries = rows(rng, 41, 16, dim, "bf16", 0.1).to("cuda:0")
+    results = []
+    for pool, last in ((need, False), ((9 << 29) // (2 * heads * page * dim), True)):
+        cache = torch.zeros((pool, 2 * heads, page, dim), dtype=torch.int8, device="cuda:0")
+        scales = torch.zeros((pool, 2 * heads, page // block), device="cuda:0")
+        pages = list(range(pool - need, pool)) if last else list(range(need))
+        table = np.full((2, 7), -1)
+        slots, at = [], 0
+        for s, n in enumerate(lengths):
+            count = -(-n // page)
+            table[s, :count] = pages[at: at + count]
+            slots += [int(table[s, i // page]) * page + i % page for i in range(n)]
+            at += count
+        assert not last or min(slots) * 2 * heads * dim > 2**32
+        quantized_cache_update(keys, values, cache, scales, int32(slots))
+        out = quantized_ragged_page_attention(queries, cache, scales, int32(lengths), int32(table), int32([0, 40, 41]), int32([2]))
+        results.append((*quantized_cache_gather(cache, scales, int32(slots)), out))
+        assert torch.isfinite(out).all() and out.abs().amax(-1).min() > 0
+        assert not last or not cache[: pool - need].any()
+    for a, b in zip(*results):
+        assert torch.equal(a, b)

@@ -185,3 +185,44 @@ def test_c_block_table_arguments():
         p = filled("RpaBlockTablesParams")
         setattr(p, field, value)
         assert lib.rpa_block_tables_launch(ctypes.byref(p), None) == -1, (field, value)
+
+
+def test_pages_of_two_gigabytes_are_refused():
+    lib = _native.load()
+    for name, entry in ENTRY.items():
+        p = filled(name)
+        p.num_kv_heads, p.page_size, p.head_dim = 128, 32768, 256  # 2**31 bytes
+        if name == "RpaQuantParams":
+            p.num_q_heads = 128
+        assert getattr(lib, entry)(ctypes.byref(p), None) == -2
+        assert b"page" in lib.rpa_last_error()
+
+
+@pytest.mark.parametrize("name", ["RpaQuantParams", "RpaQuantUpdateParams", "RpaQuantGatherParams", "RpaBlockTablesParams"])
+def test_packed_values_are_the_struct(name):
+    """Entry packs the values in order into the bytes that setting the fields one by one gives."""
+    params = getattr(_native, name)
+    p, values = params(), []
+    for k, (field, kind) in enumerate(params._fields_):
+        value = 0.5 + k if kind is ctypes.c_float else 1000 + k
+        setattr(p, field, value)
+        values.append(value)
+    entry = _native.Entry("unused", params)
+    assert entry.layout.pack(*values) == bytes(p)
+    for k, (field, kind) in enumerate(params._fields_):
+        if kind is ctypes.c_int32:
+            with pytest.raises(ValueError, match="out of range"):
+                _native.Entry("rpa_quant_fwd_launch", params)(0, *values[:k], 2**31, *values[k + 1:])
+
+
+def test_workspace_has_a_place_for_every_state_of_a_cut():
+    """Two states of a tile's rows for each of two workgroups per compute unit (256 without a device), at every width."""
+    lib = _native.load()
+    p = filled("RpaQuantParams")
+    for dim, padded, rows in ((16, 64, 192), (64, 64, 192), (96, 128, 192), (128, 128, 192), (144, 256, 64), (256, 256, 64)):
+        for dtype, own in ((_native.RPA_DTYPE_BF16, rows), (_native.RPA_DTYPE_F32, 64)):
+            p.head_dim, p.dtype = dim, dtype
+            size = lib.rpa_quant_workspace_bytes(ctypes.byref(p))
+            per_slot = (16 + own) * (padded * 4 + 8)
+            slots, rest = divmod(size - (1 << 20), per_slot)
+            assert rest == 0 and slots >= 2 * 16, (dim, dtype, size)
