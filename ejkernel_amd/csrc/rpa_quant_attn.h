@@ -26,12 +26,13 @@
 //   - decode behind a window of 4096 (64 x 4 tokens, 16/8 heads of 256): the reads, 172 us = 4.9 TB/s;
 //   - chunks: instruction issue.  A 32-key step of a 48-row wavefront at head_dim 128 is 48 matrix instructions of 16
 //     cycles and about 330 vector instructions -- 80 to widen the codes (e4m3; 210 for int8), 67 for each 16 rows' softmax,
-//     24 of them exponentials of four times the cost -- so that the vector units are busy 78 % of the time and the matrix
-//     units 33 %: 725 TFLOP/s (e4m3) and 670 (int8) for 16 chunks of 512 tokens, 775 for 2 x 8192 tokens;
+//     eight of them exponentials of four times the cost -- so that vector instructions issue in 57 % of all cycles, the matrix
+//     units are busy in 31 % and both wait for loads or each other in the rest: 730 TFLOP/s (e4m3) and 685 (int8) for 16
+//     chunks of 512 tokens, 785 for 2 x 8192 tokens;
 //   - fp32 queries: the same with three products for one and the splitting of probabilities on top: 122 TFLOP/s of plain
 //     products for a mixed batch at head_dim 96, which runs as 128;
 //   - few short sequences: the chain of dependent loads in front of the first product (lengths, their sums, page, codes),
-//     12 us for 8 sequences of up to 1024 keys.
+//     12 us for 8 sequences of up to 512 keys.
 #pragma once
 
 #include "rpa_quant.h"
