@@ -46,6 +46,7 @@ struct QuantArgs {
   int group;        // query heads per kv head
   int tile_group;   // rows of one token in a tile of the second stream: min(group, rows of a tile)
   int tile_tokens;  // tokens of a tile
+  int tile_pad;     // what a tile costs beyond its keys, in keys
   int subs;         // tiles side by side for the heads of one token, where they are more than a tile's rows
   int grid;         // workgroups, a multiple of 16
   // zero between launches: one for each workgroup's cut item of the first stream, then [level of the tree][workgroup][wavefront]
@@ -66,14 +67,17 @@ constexpr int kTileStep = 32;
 
 constexpr uint64_t kQuantTicketBytes = 1u << 18;  // of the workspace's head
 constexpr int kThinStep = 128;     // keys a workgroup takes at once in the first stream
-constexpr int kThinPad = 128;      // what an item of the first stream costs beyond its keys, in keys
-constexpr int kTilePad = 64;       // the same of the second
+// What an item costs beyond its keys, in keys: its queries, its rows' way out, a join.  First stream: 256 sequences of up to 512
+// keys take 49 us at 128, 45 at 256, 44 at 384.  Second, three row tiles: 16 chunks of 512 tokens 295 us at 64, 278 at 128,
+// 266 at 192, 264 at 256; one: a step takes a third of the time for most of the cost, yet is as well off with less (16 chunks of 1024
+// tokens at head_dim 256: 1152 us at 64, 1112 at 128, 1128 at 256).
+constexpr int kThinPad = 384;
 constexpr int kThinLeast = 256;    // least run of keys per workgroup
 constexpr int kThinUneven = 1024;  // what cuts at any place cost over cuts into equal parts, in keys of a run
 constexpr int kThinMeet = 384;     // what a cut costs at all
 constexpr int kTileLeast = 256;
 constexpr float kNoKey = -3.0e38f; // row maximum before any key
-constexpr float kLazy = 8.f;       // the running maximum follows when a logit passes it by 2^8
+constexpr float kLazy = 2048.f;    // the running maximum follows when eight probabilities under it are more than that
 constexpr int kAgentScope = 16;    // auxiliary bit of a buffer access: coherent across the device's L2s
 
 namespace quant {
@@ -109,7 +113,7 @@ __device__ __forceinline__ int tiles_of(Args& a, const Seq& q) { return (q.q_len
 // Stream positions in front of tile n (n below the number of tiles), or of all tiles.
 __device__ __forceinline__ int64_t tiles_before(Args& a, const Seq& q, int n, bool all) {
   const int base = q.kv_len - q.q_len, d = a.tile_tokens;
-  int64_t sum = ramp(n, base + d, d) + static_cast<int64_t>(n) * kTilePad;
+  int64_t sum = ramp(n, base + d, d) + static_cast<int64_t>(n) * a.tile_pad;
   if (a.p.sliding_window > 0) sum -= ramp(n, max(base - a.p.sliding_window + 1, -0x40000000), d);  // (a window beyond every key)
   if (all) sum -= max(base + n * d, 0) - max(base + q.q_len, 0);
   return sum;
@@ -135,11 +139,11 @@ __device__ __forceinline__ Seq load_seq(Args& a, int n, int s) {
 
 // A cut of a stream of `total` positions over `n` workgroups: run w is [bound(w), bound(w + 1)).  Where the whole grid takes
 // part, two workgroups share a compute unit, and the one that was there first gets the larger part of its issue slots and
-// of its memory requests: with equal runs it ends at three quarters of the other's time.  So it gets the longer run: kFirstThin or
-// kFirstTile of kPairUnits, the other the rest (2 x 8192 tokens: 865 us at 64, 816 at 76, 800 at 80; 16 chunks of 512 after
-// 4096: 304, 319 and 335; decode steps are alike from 72 to 88).  The workgroups of an XCD hold `block` neighbouring runs, those of the first
+// of its memory requests: with equal runs it ends at three quarters of the other's time.  So it gets the longer run: kFirst of
+// kPairUnits, the other the rest (2 x 8192 tokens: 746 us at 64, 724 at 72, 707 at 80; 16 chunks of 512 after 4096: 260, 255
+// and 256; decode steps of 64 x 4 tokens behind a window 173, 173 and 169, of 256 up to 8192 keys alike).  The workgroups of an XCD hold `block` neighbouring runs, those of the first
 // workgroups in front or, where `back` is set, behind.
-constexpr int kPairUnits = 128, kFirstThin = 76, kFirstTile = 78;
+constexpr int kPairUnits = 128, kFirst = 78;
 // x / y of numbers that are not negative: 32 bits nearly always; the rest bit by bit, since the code on the way to the
 // first load is fetched anew by every launch and a 64-bit division is long.
 __device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
@@ -301,6 +305,24 @@ __device__ __forceinline__ void add_sinks(Args& a, int head, float m, float& l, 
   weight = __builtin_amdgcn_exp2f(m - top);
   l *= weight;
   for (int j = 0; j < a.p.num_sinks; ++j) l += __builtin_amdgcn_exp2f(sink[j] * kLog2e - top);
+}
+
+// Register r of lane group g <-> register g of lane group r.
+template <int W>
+__device__ __forceinline__ void transpose_groups(uint32_t (&w)[4][W]) {
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const auto x = __builtin_amdgcn_permlane32_swap(w[r][k], w[r + 2][k], false, false);
+      w[r][k] = x[0], w[r + 2][k] = x[1];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r += 2) {
+      const auto x = __builtin_amdgcn_permlane16_swap(w[r][k], w[r + 1][k], false, false);
+      w[r][k] = x[0], w[r + 1][k] = x[1];
+    }
+  }
 }
 
 // N fp32 results to the output, N a multiple of 4.
@@ -521,39 +543,34 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
         }
       }
     }
-    // The largest logit of each row, from the products before their scale (scales are not negative).
-    float top[MT];
-    bool up = false;
+    // Probabilities under the running maximum as it stands.  Where some of them are so large that a logit must have passed it
+    // by far (or there was none yet), it follows, which happens a few times in a row's walk: no maximum is taken in the others.
+    bf16x8_t pf[MT][kParts];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      const float x0 = fmaxf(fmaxf(fmaxf(sa[mt][0][0], sa[mt][0][1]), sa[mt][0][2]), sa[mt][0][3]) * c[0];
-      const float x1 = fmaxf(fmaxf(fmaxf(sa[mt][1][0], sa[mt][1][1]), sa[mt][1][2]), sa[mt][1][3]) * c[1];
-      top[mt] = fmaxf(x0, x1);
-      up |= top[mt] > st.m[mt] + kLazy;
-    }
-    if (__any(up)) {
+      float pv[8], sum;
+      const auto weigh = [&] {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const float m_new = fmaxf(st.m[mt], row_groups_max(top[mt]));
+        for (int e = 0; e < 8; ++e) {
+          pv[e] = __builtin_amdgcn_exp2f(fmaf(sa[mt][e >> 2][e & 3], c[e >> 2], -st.m[mt]));
+          sum = e == 0 ? pv[0] : sum + pv[e];
+        }
+      };
+      weigh();
+      if (__any(sum > kLazy)) {
+        const float x0 = fmaxf(fmaxf(fmaxf(sa[mt][0][0], sa[mt][0][1]), sa[mt][0][2]), sa[mt][0][3]) * c[0];  // (scales are not negative)
+        const float x1 = fmaxf(fmaxf(fmaxf(sa[mt][1][0], sa[mt][1][1]), sa[mt][1][2]), sa[mt][1][3]) * c[1];
+        const float m_new = fmaxf(st.m[mt], row_groups_max(fmaxf(x0, x1)));
         const float alpha = __builtin_amdgcn_exp2f(st.m[mt] - m_new);
 #pragma unroll
         for (int n = 0; n < NO; ++n) st.acc[mt][n] *= alpha;
         st.l[mt] *= alpha;
         st.m[mt] = m_new;
+        weigh();
       }
-    }
-    bf16x8_t pf[MT][kParts];
+      st.l[mt] += sum;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      float pv[8];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(sa[mt][u][r], c[u], -st.m[mt]));
-          st.l[mt] += p;
-          pv[4 * u + r] = p * w[u];
-        }
+      for (int e = 0; e < 8; ++e) pv[e] *= w[e >> 2];
       split<kParts>(pv, pf[mt]);
     }
 #pragma unroll
@@ -800,17 +817,33 @@ __device__ __forceinline__ void tile_item(Args& a, const Seq& q, int s, int hs, 
 #pragma unroll
   for (int mt = 0; mt < kRowTiles; ++mt) {
     const Row row = row_of_tile(mt);
-    if (row.token < 0) continue;
     float weight;
-    add_sinks(a, row.head, m[mt], l[mt], weight);
+    add_sinks(a, row.token < 0 ? 0 : row.head, m[mt], l[mt], weight);
     const float f = l[mt] > 0.f ? weight / l[mt] : 0.f;
+    // A lane has four pieces of a row that follow each other; the four lanes of a row exchange them, so that a store writes
+    // whole cache lines.
+    constexpr int W = NO * static_cast<int>(sizeof(T)) / 4;
+    uint32_t w[4][W];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        if constexpr (sizeof(T) == 4) w[r][k] = __float_as_uint(acc[mt][k][r] * f);
+        else w[r][k] = pack_bf16x2(acc[mt][2 * k][r] * f, acc[mt][2 * k + 1][r] * f);
+      }
+    transpose_groups<W>(w);
+    if (row.token < 0) continue;
     T* dst = static_cast<T*>(a.p.out) + (static_cast<size_t>(q.q0 + row.token) * a.p.num_q_heads + row.head) * dim;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      float o[NO];
+      const int d = NO * (4 * r + g);
+      if (d >= dim) continue;
+      if constexpr (W == 2) {
+        *reinterpret_cast<u32x2_t*>(dst + d) = u32x2_t{w[r][0], w[r][1]};
+      } else {
 #pragma unroll
-      for (int n = 0; n < NO; ++n) o[n] = acc[mt][n][r] * f;
-      if (NO * (4 * g + r) < dim) store_row<T, NO>(dst + NO * (4 * g + r), o);
+        for (int k = 0; k < W / 4; ++k) reinterpret_cast<u32x4_t*>(dst + d)[k] = u32x4_t{w[r][4 * k], w[r][4 * k + 1], w[r][4 * k + 2], w[r][4 * k + 3]};
+      }
     }
   }
 }
@@ -903,17 +936,18 @@ __device__ __forceinline__ void tile_phase(uint64_t args) {
     const int64_t len = tiles_before(a, q, tiles, true);
     int h = static_cast<int>(divide(off, len));
     int64_t rest = off - static_cast<int64_t>(h) * len;
-    int tile = 0;
-    for (int hi = tiles; hi - tile > 1;) {  // the last tile that starts at or before the position
-      const int mid = (tile + hi) >> 1;
-      if (tiles_before(a, q, mid, false) <= rest) tile = mid;
-      else hi = mid;
+    int tile = 0;  // the last tile that starts at or before the position: 64 of them tried at once
+    for (int span = tiles; span > 1;) {
+      const int step = (span + 63) >> 6, k = static_cast<int>(threadIdx.x & 63) * step;
+      const int before = __popcll(__ballot(k < span && tiles_before(a, q, tile + min(k, span - 1), false) <= rest)) - 1;
+      tile += before * step;
+      span = min(step, span - before * step);
     }
     int begin = static_cast<int>(rest - tiles_before(a, q, tile, false));
     for (; h < heads && x < run.x_end; ++h, tile = 0) {
       for (; tile < tiles && x < run.x_end; ++tile, begin = 0) {
         const Range range = key_range(a, q, tile * a.tile_tokens, min((tile + 1) * a.tile_tokens, q.q_len));
-        const int keys = range.end - range.first, all = range.end - (range.first & ~31), item = keys + kTilePad;
+        const int keys = range.end - range.first, all = range.end - (range.first & ~31), item = keys + a.tile_pad;
         const int end = static_cast<int>(min(static_cast<int64_t>(item), begin + (run.x_end - x)));
         const int ka = begin >= keys ? all : begin / kStep * kStep, kb = end >= keys ? all : end / kStep * kStep;
         if (ka < kb || (keys == 0 && begin == 0))
@@ -1006,7 +1040,7 @@ __global__ __launch_bounds__(256, 2) void quant_attention_kernel(QuantArgs) {
     r.cut.n = whole ? a.grid : static_cast<int>(r.fixed > 0 ? items * parts : min(most, static_cast<int64_t>(a.grid / 2)));
     r.cut.block = whole ? a.grid / 8 : 2 * r.cut.n;
     r.cut.pair = whole ? kPairUnits : 2;
-    r.cut.lead = !whole ? 1 : c == 0 ? kFirstThin : kPairUnits - kFirstTile;
+    r.cut.lead = !whole ? 1 : c == 0 ? kFirst : kPairUnits - kFirst;
     r.cut.set(total[c]);
     // the first stream from the grid's front, the second from its back: where both are short they meet different workgroups
     r.self = total[c] > 0 ? place_in_cut(c == 0 ? blockIdx.x : a.grid - 1 - blockIdx.x, r.cut.n) : -1;
