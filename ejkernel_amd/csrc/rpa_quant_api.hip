@@ -10,11 +10,14 @@ namespace {
 bool aligned_to(const void* ptr, uint32_t bytes) { return (reinterpret_cast<uintptr_t>(ptr) & (bytes - 1)) == 0; }
 bool power_of_two(int32_t x) { return x > 0 && (x & (x - 1)) == 0; }
 
+constexpr int32_t kMostCount = 1 << 30;  // of tokens, requests and places: sums of two and rounding up stay in 32 bits
+
 // Shape of the pool; the same for the attention, the update and the read-back.
 template <typename P>
 int check_pool(const P& p) {
   if (p.total_tokens < 0 || p.num_kv_heads <= 0 || p.num_pages <= 0)
     return fail(RPA_ERR_INVALID_ARGUMENT, "non-positive dimension");
+  if (p.total_tokens > kMostCount) return fail(RPA_ERR_UNSUPPORTED, "total_tokens=%d: at most 2^30", p.total_tokens);
   if (p.num_kv_heads > 16384) return fail(RPA_ERR_UNSUPPORTED, "num_kv_heads=%d: at most 16384", p.num_kv_heads);
   if (p.head_dim < 16 || p.head_dim > 256 || p.head_dim % 16 != 0)
     return fail(RPA_ERR_UNSUPPORTED, "head_dim=%d must be a multiple of 16 from 16 to 256", p.head_dim);
@@ -43,6 +46,7 @@ int check_attention(const RpaQuantParams& p) {
   if (rc != RPA_OK) return rc;
   if (p.num_q_heads <= 0 || p.max_num_seqs <= 0 || p.pages_per_seq <= 0 || p.num_sinks < 0)
     return fail(RPA_ERR_INVALID_ARGUMENT, "non-positive dimension in RpaQuantParams");
+  if (p.max_num_seqs > kMostCount) return fail(RPA_ERR_UNSUPPORTED, "max_num_seqs=%d: at most 2^30", p.max_num_seqs);
   if (p.num_q_heads % p.num_kv_heads != 0)
     return fail(RPA_ERR_INVALID_ARGUMENT, "num_q_heads=%d must be divisible by num_kv_heads=%d", p.num_q_heads, p.num_kv_heads);
   if (static_cast<int64_t>(p.pages_per_seq) * p.page_size > (1 << 30))
@@ -147,6 +151,8 @@ int rpa_block_tables_launch(const RpaBlockTablesParams* params, void* hip_stream
     const RpaBlockTablesParams& p = *params;
     if (p.max_num_seqs <= 0 || p.pages_per_seq <= 0 || p.num_free_slots <= 0 || p.page_size <= 0 || p.total_tokens < 0)
       return rpa::fail(RPA_ERR_INVALID_ARGUMENT, "non-positive dimension in RpaBlockTablesParams");
+    if (p.max_num_seqs > rpa::kMostCount || p.num_free_slots > rpa::kMostCount || p.total_tokens > rpa::kMostCount)
+      return rpa::fail(RPA_ERR_UNSUPPORTED, "max_num_seqs=%d, num_free_slots=%d and total_tokens=%d: at most 2^30 each", p.max_num_seqs, p.num_free_slots, p.total_tokens);
     const void* ptrs[] = {p.query_lens, p.cached_lens, p.block_tables, p.free_pages, p.free_state, p.num_seqs, p.query_start_loc,
                           p.context_lens, p.admitted, p.cached_lens_out, p.free_state_out, p.scratch};
     for (const void* q : ptrs)

@@ -289,8 +289,8 @@ int rpa_ragged_decode_launch(const RpaRaggedDecodeParams* params, void* hip_stre
  *   kv_scales [num_pages, 2*num_kv_heads, page_size / scale_block] fp32, not negative; element = code * scale of its block.
  *
  * head_dim is a multiple of 16 from 16 to 256, page_size a power of two from 4 to 32768, scale_block a power of two from 4
- * to page_size, num_pages * page_size below 2^31, a page smaller than 2^31 bytes, pages_per_seq * page_size at most 2^30.
- * Slot = page * page_size + offset names a token's place in the pool.
+ * to page_size, num_pages * page_size below 2^31, a page smaller than 2^31 bytes, pages_per_seq * page_size,
+ * total_tokens and max_num_seqs at most 2^30.  Slot = page * page_size + offset names a token's place in the pool.
  */
 
 /* Attention over that cache: queries of every sequence against its keys, causal from the end of its context, with the
@@ -386,7 +386,8 @@ int rpa_quant_gather_launch(const RpaQuantGatherParams* params, void* hip_stream
  *   query_lens[s] == 0  it idles: nothing changes.
  *   query_lens[s] < 0   it has ended: its pages go back to the ring (behind the free ones, in the order of its table).
  * block_tables and free_pages are updated in place; entries of a table behind a request's pages keep what they hold.
- * Page ids are taken as they stand.  Sequences from num_seqs on have no tokens, a context of 0 and keep their cached_lens. */
+ * Page ids are taken as they stand.  max_num_seqs,
+ * num_free_slots and total_tokens are at most 2^30.  Sequences from num_seqs on have no tokens, a context of 0 and keep their cached_lens. */
 typedef struct RpaBlockTablesParams {
   const int32_t* query_lens;      /* [max_num_seqs] */
   const int32_t* cached_lens;     /* [max_num_seqs] tokens in the cache before this step */

@@ -226,3 +226,13 @@ def test_workspace_has_a_place_for_every_state_of_a_cut():
             per_slot = (16 + own) * (padded * 4 + 8)
             slots, rest = divmod(size - (1 << 20), per_slot)
             assert rest == 0 and slots >= 2 * 16, (dim, dtype, size)
+
+
+def test_counts_beyond_2_30_are_refused():
+    lib = _native.load()
+    for name, entry in (*ENTRY.items(), ("RpaBlockTablesParams", "rpa_block_tables_launch")):
+        for field in ("total_tokens", "max_num_seqs", "num_free_slots"):
+            p = filled(name)
+            if hasattr(p, field):
+                setattr(p, field, (1 << 30) + 1)
+                assert getattr(lib, entry)(ctypes.byref(p), None) == -2, (name, field, lib.rpa_last_error())
