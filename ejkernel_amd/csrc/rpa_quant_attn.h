@@ -58,11 +58,23 @@ struct QuantArgs {
   float* tile_ml;           // [2 * grid][rows][2]
 };
 
-// The second stream's tiles for a (padded) head_dim: 16-row tiles per wavefront, and keys per step.  Three share the
-// widening of a key among 48 rows in what registers there are at two workgroups per compute unit; head_dim 256 has room for
-// one, and so have fp32 queries (two spill: 113 in place of 104 us for a mixed batch at head_dim 96).
+// The second stream's tiles for a (padded) head_dim: 16-row tiles per wavefront, and keys per step.  The more of them, the more
+// rows share the widening of a key: as many as there are registers for at two workgroups per compute unit, for which some of the
+// queries lie in LDS.  16 chunks of 1024 tokens at head_dim 256: 1088 us with one, 711 with two; 16 of 512 at 64: 356 us with
+// three, 342 with four; in fp32 at 128: 670 us with one, 567 with two; at 128 four spill (332 us, three 257).
 template <int D, int kParts>
-constexpr int quant_row_tiles() { return kParts == 3 || D == 256 ? 1 : 3; }
+constexpr int quant_row_tiles() { return kParts == 3 ? (D == 256 ? 1 : 2) : D == 256 ? 2 : D == 128 ? 3 : 4; }
+// The queries that stay in registers: of a row's pieces of 32 elements the first so many, and of their bf16 parts.  The others
+// are read from LDS for every step.  At head_dim 128 all in registers spill outside of the loops (decode of 256 sequences 424 us, 16
+// chunks of 512 tokens 258 us), half of the pieces do not (411 and 257 us), none cost the loop more reads (411 and 266 us).
+template <int D, int kParts>
+constexpr int quant_reg_pieces() { return D == 128 && kParts == 1 ? 2 : D / 32; }
+template <int D, int kParts>
+constexpr int quant_reg_parts() { return D == 256 && kParts == 1 ? 0 : D == 128 && kParts == 3 ? 1 : kParts; }
+// Whether the second stream is a function of its own: it then has the whole register file at the price of a few us at its
+// start.  At head_dim 256 its spills would cost the first stream more (64 x 4 tokens behind a window: 195 us against 175).
+template <int D, int kParts>
+constexpr bool quant_apart() { return D == 256 && kParts == 1; }
 constexpr int kTileStep = 32;
 
 constexpr uint64_t kQuantTicketBytes = 1u << 18;  // of the workspace's head
@@ -390,8 +402,8 @@ struct RowState {
   f32x4_t acc[MT][kD / 16];  // output element (kD / 16) (4 g + r) + n of row i, unnormalised
   float m[MT], l[MT];        // running maximum (log2) of the row, this lane's share of its sum
 };
-template <int kCode, int D, int kParts, bool kCap, bool kWide, int MT>
-__device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const bf16x8_t (&qf)[MT][D / 32][kParts],
+template <int kCode, int D, int kParts, bool kCap, bool kWide, int MT, typename Q>
+__device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const Q& query,
                                      const int (&hi)[MT], const Range& range, int full_lo, int full_hi, int k_begin, int k_end, int stride,
                                      RowState<MT, D>& st) {
   constexpr int NP = D / 64, NV = D / 64, NO = D / 16;
@@ -445,18 +457,23 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
   const char* v_rows[2];    // where V of the tile in flight begins, and its scales: known when its K was asked for
   const float* v_scale[2];
   auto load_k = [&](int k0, const Pages& pg) {
+    const char* rows[2];
+    const float* sc[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       // the pages are clamped here, where they are used, so that nothing waits for them where they are loaded
       const int page = clamp_page(pg.k[u], a.p.num_pages), v_page = kWide ? page : clamp_page(pg.v[u], a.p.num_pages);
-      const char* row = codes_at(page, k0 + 16 * u + (kWide ? 0 : i));
-      const float* sc = scales_at(v_page, k0 + 16 * u + (kWide ? 0 : 4 * g));
-      v_rows[u] = (kWide ? row : codes_at(v_page, k0 + 16 * u + 4 * g)) + head_bytes;
-      v_scale[u] = sc + head_scales;
-#pragma unroll
-      for (int n = 0; n < NP; ++n) kr[u][n] = *reinterpret_cast<const u32x4_t*>(row + here(k_off[n]));
-      ks[u] = kWide ? sc[here(sc_off)] : *sc;
+      rows[u] = codes_at(page, k0 + 16 * u + (kWide ? 0 : i));
+      sc[u] = scales_at(v_page, k0 + 16 * u + (kWide ? 0 : 4 * g));
+      v_rows[u] = (kWide ? rows[u] : codes_at(v_page, k0 + 16 * u + 4 * g)) + head_bytes;
+      v_scale[u] = sc[u] + head_scales;
     }
+#pragma unroll
+    for (int n = 0; n < NP; ++n)  // in the order of their use
+#pragma unroll
+      for (int u = 0; u < 2; ++u) kr[u][n] = *reinterpret_cast<const u32x4_t*>(rows[u] + here(k_off[n]));
+#pragma unroll
+    for (int u = 0; u < 2; ++u) ks[u] = kWide ? sc[u][here(sc_off)] : *sc[u];
   };
   auto load_v = [&] {
 #pragma unroll
@@ -494,18 +511,21 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) sa[mt][0] = sa[mt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int n = 0; n < NP; ++n) {
+      bf16x8_t op[2][2];
 #pragma unroll
-      for (int n = 0; n < NP; ++n) {
-        bf16x8_t op[2];
-        widen16<kCode>(kr[u][n], op);
+      for (int u = 0; u < 2; ++u) widen16<kCode>(kr[u][n], op[u]);
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
+      for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int sp = 0; sp < kParts; ++sp) sa[mt][u] = mfma(op[hf], qf[mt][2 * n + hf][sp], sa[mt][u]);
-      }
+          for (int sp = 0; sp < kParts; ++sp) {
+            const bf16x8_t x = query(mt, 2 * n + hf, sp);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) sa[mt][u] = mfma(op[u][hf], x, sa[mt][u]);
+          }
+    }
     float c[2] = {ks[0] * c_scale, ks[1] * c_scale}, w[2] = {vs[0], vs[1]};
     const bool more = k0 + stride < k_end;
     const int ahead = more ? k0 + stride : k0;
@@ -629,7 +649,7 @@ __device__ __forceinline__ void thin_item(Args& a, const Seq& q, int s, int h, i
     for (int k = 0; k < D / 32; ++k) load_q<T, kParts>(a, row, real, 16 * (g + 4 * (k >> 1)) + 8 * (k & 1), qf[0][k]);
   }
   RowState<1, D> st;
-  walk<kCode, D, kParts, kCap, kWide, 1>(a, q, s, h, qf, {hi}, range, full_lo, full_hi, base + ka + 32 * wave, base + ((min(kb, keys) + 31) & ~31), 128, st);
+  walk<kCode, D, kParts, kCap, kWide, 1>(a, q, s, h, [&](int, int k, int sp) { return qf[0][k][sp]; }, {hi}, range, full_lo, full_hi, base + ka + 32 * wave, base + ((min(kb, keys) + 31) & ~31), 128, st);
   const auto& acc = st.acc[0];
   const float m = st.m[0], l = st.l[0];
 
@@ -713,9 +733,22 @@ __device__ __forceinline__ void thin_item(Args& a, const Seq& q, int s, int h, i
   if (NO * (4 * g + wave) < dim) store_row<T, NO>(dst + NO * (4 * g + wave), o);
 }
 
+// Queries of a tile that are not in registers: every wavefront's own, as the matrix unit takes them.
+template <int D, int kParts>
+struct TileLds {
+  static constexpr bool kAllParts = quant_reg_pieces<D, kParts>() < D / 32;  // of the pieces behind the first, else the last parts of all
+  static constexpr int kPieces = kAllParts ? D / 32 - quant_reg_pieces<D, kParts>() : D / 32;
+  static constexpr int kLds = kAllParts ? kParts : kParts - quant_reg_parts<D, kParts>();
+  bf16x8_t q[4][quant_row_tiles<D, kParts>()][kPieces][kLds > 0 ? kLds : 1][kLds > 0 ? 64 : 1];
+  __device__ __forceinline__ bf16x8_t& at(int wave, int mt, int k, int sp) {
+    return q[wave][mt][k - (D / 32 - kPieces)][kAllParts ? sp : sp - (kParts - kLds)][threadIdx.x & 63];
+  }
+};
+
 // A run of keys [ka, kb) of one tile of rows.
 template <int kCode, int D, typename T, int kParts, bool kCap, bool kWide>
-__device__ __forceinline__ void tile_item(Args& a, const Seq& q, int s, int hs, int tile, int ka, int kb, const Cut& cut, int self, int64_t x0) {
+__device__ __forceinline__ void tile_item(Args& a, const Seq& q, int s, int hs, int tile, int ka, int kb, const Cut& cut, int self, int64_t x0,
+                                          TileLds<D, kParts>& lds) {
   constexpr int kRowTiles = quant_row_tiles<D, kParts>(), NO = D / 16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
   const int dim = a.p.head_dim;
@@ -735,7 +768,8 @@ __device__ __forceinline__ void tile_item(Args& a, const Seq& q, int s, int hs, 
     return Row{dt < t1 - t0 && gg < a.group ? t0 + dt : -1, h * a.group + gg};
   };
   int hi[kRowTiles];
-  bf16x8_t qf[kRowTiles][D / 32][kParts];
+  constexpr int kReg = quant_reg_parts<D, kParts>(), kPieces = quant_reg_pieces<D, kParts>();
+  bf16x8_t qf[kRowTiles][D / 32][kReg > 0 ? kReg : 1];
 #pragma unroll
   for (int mt = 0; mt < kRowTiles; ++mt) {
     const Row row = row_of_tile(mt);
@@ -743,12 +777,21 @@ __device__ __forceinline__ void tile_item(Args& a, const Seq& q, int s, int hs, 
     hi[mt] = real ? q_base + row.token + 1 : 0;
     const T* src = static_cast<const T*>(a.p.queries) + (q.q0 + (real ? row.token : 0)) * a.p.query_token_stride + (real ? row.head : 0) * a.p.query_head_stride;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) load_q<T, kParts>(a, src, real, 16 * (g + 4 * (k >> 1)) + 8 * (k & 1), qf[mt][k]);
+    for (int k = 0; k < D / 32; ++k) {
+      bf16x8_t part[kParts];
+      load_q<T, kParts>(a, src, real, 16 * (g + 4 * (k >> 1)) + 8 * (k & 1), part);
+#pragma unroll
+      for (int sp = 0; sp < kParts; ++sp) {
+        if (sp < kReg && k < kPieces) qf[mt][k][sp] = part[sp];
+        else lds.at(wave, mt, k, sp) = part[sp];
+      }
+    }
   }
+  const auto query = [&](int mt, int k, int sp) { return sp < kReg && k < kPieces ? qf[mt][k][sp] : lds.at(wave, mt, k, sp); };
   const int full_lo = a.p.sliding_window > 0 ? max(q_base + t1 - a.p.sliding_window, 0) : 0;  // keys every row sees
   const int full_hi = q_base + t0 + 1;
   RowState<kRowTiles, D> st;
-  walk<kCode, D, kParts, kCap, kWide, kRowTiles>(a, q, s, h, qf, hi, range, full_lo, full_hi, base + ka, base + ((min(kb, keys) + 31) & ~31), 32, st);
+  walk<kCode, D, kParts, kCap, kWide, kRowTiles>(a, q, s, h, query, hi, range, full_lo, full_hi, base + ka, base + ((min(kb, keys) + 31) & ~31), 32, st);
   auto& acc = st.acc;
   auto& m = st.m;
   auto& l = st.l;
@@ -870,15 +913,18 @@ struct SchedLds {
   int flag;
 };
 
-template <int D>
+template <int D, int kParts>
 struct Lds {
-  ThinLds<D> thin;
+  union {
+    ThinLds<D> thin;
+    TileLds<D, kParts> tile;
+  };
   SchedLds sched;
 };
-template <int D>
-__device__ __forceinline__ Lds<D>& lds_of() {
-  __shared__ __align__(16) char bytes[sizeof(Lds<D>)];
-  return *reinterpret_cast<Lds<D>*>(bytes);
+template <int D, int kParts>
+__device__ __forceinline__ Lds<D, kParts>& lds_of() {
+  __shared__ __align__(16) char bytes[sizeof(Lds<D, kParts>)];
+  return *reinterpret_cast<Lds<D, kParts>*>(bytes);
 }
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -895,7 +941,7 @@ __device__ __forceinline__ Run uniform(const Run& r) {
 template <int kCode, int D, typename T, int kParts, bool kCap, bool kWide>
 __device__ __forceinline__ void thin_phase(uint64_t args) {
   Args& a = *reinterpret_cast<Args*>(uniform(static_cast<int64_t>(args)));
-  Lds<D>& lds = lds_of<D>();
+  Lds<D, kParts>& lds = lds_of<D, kParts>();
   const Run run = uniform(lds.sched.run[0]);
   Window window;
   int s = run.seq;
@@ -924,8 +970,9 @@ template <int kCode, int D, typename T, int kParts, bool kCap, bool kWide>
 __device__ __forceinline__ void tile_phase(uint64_t args) {
   constexpr int kStep = kTileStep;
   Args& a = *reinterpret_cast<Args*>(uniform(static_cast<int64_t>(args)));
-  Lds<D>& lds = lds_of<D>();
+  Lds<D, kParts>& lds = lds_of<D, kParts>();
   const Run run = uniform(lds.sched.run[1]);
+  __syncthreads();  // the other stream's items may still be read from LDS
   Window window;
   int s = run.seq;
   int64_t off = run.off, x = run.x;
@@ -951,7 +998,7 @@ __device__ __forceinline__ void tile_phase(uint64_t args) {
         const int end = static_cast<int>(min(static_cast<int64_t>(item), begin + (run.x_end - x)));
         const int ka = begin >= keys ? all : begin / kStep * kStep, kb = end >= keys ? all : end / kStep * kStep;
         if (ka < kb || (keys == 0 && begin == 0))
-          tile_item<kCode, D, T, kParts, kCap, kWide>(a, q, s, h, tile, keys == 0 ? 0 : ka, kb, run.cut, run.self, x - begin);
+          tile_item<kCode, D, T, kParts, kCap, kWide>(a, q, s, h, tile, keys == 0 ? 0 : ka, kb, run.cut, run.self, x - begin, lds.tile);
         x += end - begin;
       }
     }
@@ -962,9 +1009,14 @@ __device__ __forceinline__ void tile_phase(uint64_t args) {
 }
 
 template <int kCode, int D, typename T, int kParts, bool kCap, bool kWide>
+__device__ __attribute__((noinline)) void tile_phase_apart(uint64_t args) {
+  tile_phase<kCode, D, T, kParts, kCap, kWide>(args);
+}
+
+template <int kCode, int D, typename T, int kParts, bool kCap, bool kWide>
 __global__ __launch_bounds__(256, 2) void quant_attention_kernel(QuantArgs) {
   Args& a = *(Args*)__builtin_amdgcn_kernarg_segment_ptr();
-  SchedLds& sched = lds_of<D>().sched;
+  SchedLds& sched = lds_of<D, kParts>().sched;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n = min(max(a.p.num_seqs[0], 0), a.p.max_num_seqs);
 
@@ -1072,7 +1124,10 @@ __global__ __launch_bounds__(256, 2) void quant_attention_kernel(QuantArgs) {
     const int c = (k == 0) == thin_first ? 0 : 1;
     const uint64_t args = reinterpret_cast<uint64_t>(&a);
     if (c == 0 && has[0]) thin_phase<kCode, D, T, kParts, kCap, kWide>(args);
-    if (c == 1 && has[1]) tile_phase<kCode, D, T, kParts, kCap, kWide>(args);
+    if (c == 1 && has[1]) {
+      if constexpr (quant_apart<D, kParts>()) tile_phase_apart<kCode, D, T, kParts, kCap, kWide>(args);
+      else tile_phase<kCode, D, T, kParts, kCap, kWide>(args);
+    }
   }
 
   // Rows in front of the first sequence and behind the last are zeros.

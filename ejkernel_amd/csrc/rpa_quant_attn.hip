@@ -49,7 +49,7 @@ int launch_quant_attention(const RpaQuantParams& p, hipStream_t stream) {
   a.tile_tokens = rows / a.tile_group;
   a.subs = (a.group + rows - 1) / rows;
   if (a.subs > 1) a.tile_tokens = 1;
-  a.tile_pad = rows > 64 ? 224 : 112;
+  a.tile_pad = rows > 128 ? 224 : rows > 64 ? 160 : 112;
   a.grid = grid_of();
   int levels = 0;
   while ((1 << levels) < a.grid) ++levels;

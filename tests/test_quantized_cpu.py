@@ -216,11 +216,11 @@ def test_packed_values_are_the_struct(name):
 
 
 def test_workspace_has_a_place_for_every_state_of_a_cut():
-    """Two states of a tile's rows for each of two workgroups per compute unit (256 without a device), at every width."""
+    """Two states of a tile's rows for each of two workgroups per compute unit, at every width: rows are bf16, fp32."""
     lib = _native.load()
     p = filled("RpaQuantParams")
-    for dim, padded, rows in ((16, 64, 192), (64, 64, 192), (96, 128, 192), (128, 128, 192), (144, 256, 64), (256, 256, 64)):
-        for dtype, own in ((_native.RPA_DTYPE_BF16, rows), (_native.RPA_DTYPE_F32, 64)):
+    for dim, padded, rows in ((16, 64, (256, 128)), (64, 64, (256, 128)), (96, 128, (192, 128)), (128, 128, (192, 128)), (144, 256, (128, 64)), (256, 256, (128, 64))):
+        for dtype, own in zip((_native.RPA_DTYPE_BF16, _native.RPA_DTYPE_F32), rows):
             p.head_dim, p.dtype = dim, dtype
             size = lib.rpa_quant_workspace_bytes(ctypes.byref(p))
             per_slot = (16 + own) * (padded * 4 + 8)
