@@ -13,7 +13,7 @@
 // tiles of rows, an item each of the second stream: each wavefront has rows of its own (quant_row_tiles times 16) and walks
 // all of the item's keys.  In both a wavefront loads K and V straight into the registers that the matrix unit takes them
 // from, so nothing waits for another wavefront on the way (with the tiles' codes widened through LDS, the workgroup in
-// step, 16 chunks of 512 tokens after 4096 took 410 us; so, 295 to 320 us).
+// step, 16 chunks of 512 tokens after 4096 took 410 us, without it 315 us as it then stood).
 //
 // Each stream is cut into equal runs of keys, one per workgroup, wherever the cut falls: few long sequences, one long chunk
 // and a ragged batch all fill the device.  Parts of an item that is cut meet through the workspace: those of the first
@@ -22,14 +22,14 @@
 // first, so that one workgroup of a compute unit waits for memory while the other multiplies.
 //
 // What bounds it, on a device that copies at 4.9 TB/s, reads at 6.2 TB/s and multiplies bf16 matrices at 1325 TFLOP/s:
-//   - decode, 256 sequences of up to 8192 keys, 32/8 heads of 128: the reads, 2.3 GB in 423 us = 5.5 TB/s;
-//   - decode behind a window of 4096 (64 x 4 tokens, 16/8 heads of 256): the reads, 172 us = 4.9 TB/s;
+//   - decode, 256 sequences of up to 8192 keys, 32/8 heads of 128: the reads, 2.3 GB in 413 us = 5.6 TB/s;
+//   - decode behind a window of 4096 (64 x 4 tokens, 16/8 heads of 256): the reads, 174 us = 4.8 TB/s;
 //   - chunks: instruction issue.  A 32-key step of a 48-row wavefront at head_dim 128 is 48 matrix instructions of 16
-//     cycles and about 330 vector instructions -- 80 to widen the codes (e4m3; 210 for int8), 67 for each 16 rows' softmax,
-//     eight of them exponentials of four times the cost -- so that vector instructions issue in 57 % of all cycles, the matrix
-//     units are busy in 31 % and both wait for loads or each other in the rest: 730 TFLOP/s (e4m3) and 685 (int8) for 16
-//     chunks of 512 tokens, 785 for 2 x 8192 tokens;
-//   - fp32 queries: the same with three products for one and the splitting of probabilities on top: 122 TFLOP/s of plain
+//     cycles and about 300 vector instructions -- 80 to widen the codes (e4m3; 210 for int8), 60 for each 16 rows' softmax,
+//     eight of them exponentials of four times the cost -- so that vector instructions issue in 61 % of all cycles, the matrix
+//     units are busy in 37 % and both wait for loads or each other in the rest: 820 TFLOP/s (e4m3) and 720 (int8) for 16
+//     chunks of 512 tokens, 830 for 2 x 8192 tokens;
+//   - fp32 queries: the same with three products for one and the splitting of probabilities on top: 125 TFLOP/s of plain
 //     products for a mixed batch at head_dim 96, which runs as 128;
 //   - few short sequences: the chain of dependent loads in front of the first product (lengths, their sums, page, codes),
 //     12 us for 8 sequences of up to 512 keys.
@@ -81,8 +81,8 @@ constexpr uint64_t kQuantTicketBytes = 1u << 18;  // of the workspace's head
 constexpr int kThinStep = 128;     // keys a workgroup takes at once in the first stream
 // What an item costs beyond its keys, in keys: its queries, its rows' way out, a join.  First stream: 256 sequences of up to 512
 // keys take 49 us at 128, 45 at 256, 44 at 384.  Second, three row tiles: 16 chunks of 512 tokens 295 us at 64, 278 at 128,
-// 266 at 192, 264 at 256; one: a step takes a third of the time for most of the cost, yet is as well off with less (16 chunks of 1024
-// tokens at head_dim 256: 1152 us at 64, 1112 at 128, 1128 at 256).
+// 266 at 192, 264 at 256, so 224 for three and four; with one a step takes less time but so does the rest (16 chunks of 1024 tokens at
+// head_dim 256: 1152 us at 64, 1112 at 128, 1128 at 256): 112, and 160 for two (QuantArgs::tile_pad).
 constexpr int kThinPad = 384;
 constexpr int kThinLeast = 256;    // least run of keys per workgroup
 constexpr int kThinUneven = 1024;  // what cuts at any place cost over cuts into equal parts, in keys of a run
