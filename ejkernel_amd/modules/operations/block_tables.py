@@ -55,8 +55,8 @@ class BuildBlockTables:
             raise ValueError(f"page_size={page_size} must be positive and below 2**31")
         if not 0 <= total_tokens <= 2**30:
             raise ValueError(f"total_tokens={total_tokens} must be from 0 to 2**30")
-        index = _on_device("build_block_tables", block_tables, query_lens=query_lens, cached_lens=cached_lens,
-                           free_pages=free_pages, free_state=free_state, num_seqs=num_seqs)
+        index = _on_device("build_block_tables", ("block_tables", block_tables), ("query_lens", query_lens), ("cached_lens", cached_lens),
+                           ("free_pages", free_pages), ("free_state", free_state), ("num_seqs", num_seqs))
         query_lens, cached_lens, free_state = query_lens.contiguous(), cached_lens.contiguous(), free_state.contiguous()
 
         # one allocation: the kernels' scratch, at the allocator's alignment, and a view for each result

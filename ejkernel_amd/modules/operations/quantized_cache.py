@@ -32,12 +32,13 @@ _current_device = torch._C._cuda_getDevice
 
 def _check_cache(kv_cache, kv_scales) -> tuple[int, int, int, int, int, int]:
     """Checks the two arrays against each other; returns the shape of the cache, the tokens a scale covers and the type's code."""
-    if kv_cache.dim() != 4:
-        raise ValueError(f"kv_cache must be [num_pages, 2 * num_kv_heads, page_size, head_dim], got {tuple(kv_cache.shape)}")
+    shape = kv_cache.shape
+    if len(shape) != 4:
+        raise ValueError(f"kv_cache must be [num_pages, 2 * num_kv_heads, page_size, head_dim], got {tuple(shape)}")
     code = _CACHE_DTYPES.get(kv_cache.dtype)
     if code is None:
         raise ValueError(f"kv_cache.dtype={kv_cache.dtype} must be int8, float8_e4m3fn or float8_e5m2")
-    num_pages, heads, page_size, head_dim = kv_cache.shape
+    num_pages, heads, page_size, head_dim = shape
     if heads % 2 != 0 or heads == 0:
         raise ValueError(f"kv_cache.shape[1]={heads} must be 2 * num_kv_heads")
     shape = kv_scales.shape
@@ -51,20 +52,23 @@ def _check_cache(kv_cache, kv_scales) -> tuple[int, int, int, int, int, int]:
     return num_pages, heads, page_size, head_dim, page_size // blocks, code
 
 
-def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
-    """``[tokens, heads, head_dim]`` as the kernels read it in place, rows of 16-byte pieces, with its strides between tokens
-    and heads; anything else is copied."""
+def _rows(t: torch.Tensor, shape) -> tuple[torch.Tensor, int, int, int]:
+    """``[tokens, heads, head_dim]`` as the kernels read it in place, rows of 16-byte pieces, with its address and its strides
+    between tokens and heads; anything else is copied."""
+    address = t.data_ptr()
+    if address % 16 == 0 and t.is_contiguous():  # (head_dim is checked behind the C entry)
+        return t, address, shape[1] * shape[2], shape[2]
     unit = 16 // t.element_size()
     for _ in range(3):
         token, head, element = t.stride()
-        if t.shape[0] <= 1:
+        if shape[0] <= 1:
             token = 0
-        if t.shape[1] <= 1:
+        if shape[1] <= 1:
             head = 0
         if element == 1 and token % unit == 0 and head % unit == 0 and t.data_ptr() % 16 == 0:
             break
         t = t.clone() if t.is_contiguous() else t.contiguous()
-    return t, token, head
+    return t, t.data_ptr(), token, head
 
 
 def _check_index_arrays(*arrays: tuple[str, torch.Tensor, int]) -> None:
@@ -76,12 +80,13 @@ def _check_index_arrays(*arrays: tuple[str, torch.Tensor, int]) -> None:
             raise ValueError(f"{name}.dtype={t.dtype} must be int32")
 
 
-def _on_device(op: str, first: torch.Tensor, **others: torch.Tensor) -> int:
+def _on_device(op: str, *tensors: tuple[str, torch.Tensor]) -> int:
     """Index of the device that all of the tensors are on."""
-    if not first.is_cuda:
-        raise RuntimeError(f"{op} needs tensors on a ROCm device (gfx950); there is no CPU implementation in this package.")
+    first = tensors[0][1]
     index = first.get_device()
-    for name, t in others.items():
+    if index < 0:
+        raise RuntimeError(f"{op} needs tensors on a ROCm device (gfx950); there is no CPU implementation in this package.")
+    for name, t in tensors:
         if t.get_device() != index:
             raise ValueError(f"{name} is on {t.device}, expected {first.device}")
     return index
@@ -111,17 +116,17 @@ class QuantizedCacheUpdate:
         if dtype is None or values.dtype != keys.dtype:
             raise ValueError(f"keys and values must share one dtype, bfloat16 or float32, got {keys.dtype} and {values.dtype}")
         tokens = shape[0]
-        if slot_mapping.dim() != 1 or slot_mapping.shape[0] != tokens or slot_mapping.dtype != torch.int32:
+        if slot_mapping.shape != (tokens,) or slot_mapping.dtype != torch.int32:
             raise ValueError(f"slot_mapping must be int32 [{tokens}], got {slot_mapping.dtype} {tuple(slot_mapping.shape)}")
         if keys.requires_grad or values.requires_grad or kv_scales.requires_grad:
             raise NotImplementedError("quantized_cache_update is forward-only; detach the inputs")
-        index = _on_device("quantized_cache_update", kv_cache, keys=keys, values=values, kv_scales=kv_scales, slot_mapping=slot_mapping)
+        index = _on_device("quantized_cache_update", ("kv_cache", kv_cache), ("keys", keys), ("values", values), ("kv_scales", kv_scales), ("slot_mapping", slot_mapping))
         if tokens == 0:
             return kv_cache, kv_scales
-        keys, key_token, key_head = _rows(keys)
-        values, value_token, value_head = _rows(values)
+        keys, key_address, key_token, key_head = _rows(keys, shape)
+        values, value_address, value_token, value_head = _rows(values, shape)
         slot_mapping = slot_mapping.contiguous()
-        _call(self._entry, index, keys.data_ptr(), values.data_ptr(), kv_cache.data_ptr(), kv_scales.data_ptr(), slot_mapping.data_ptr(),
+        _call(self._entry, index, key_address, value_address, kv_cache.data_ptr(), kv_scales.data_ptr(), slot_mapping.data_ptr(),
               key_token, key_head, value_token, value_head, tokens, heads // 2, head_dim, page_size, block, num_pages, dtype, code)
         return kv_cache, kv_scales
 
@@ -141,7 +146,7 @@ class QuantizedCacheGather:
             raise ValueError(f"slot_mapping must be int32 [total_tokens], got {slot_mapping.dtype} {tuple(slot_mapping.shape)}")
         if kv_scales.requires_grad:
             raise NotImplementedError("quantized_cache_gather is forward-only; detach the inputs")
-        index = _on_device("quantized_cache_gather", kv_cache, kv_scales=kv_scales, slot_mapping=slot_mapping)
+        index = _on_device("quantized_cache_gather", ("kv_cache", kv_cache), ("kv_scales", kv_scales), ("slot_mapping", slot_mapping))
         tokens = slot_mapping.shape[0]
         shape = (tokens, heads // 2, head_dim)
         keys = kv_scales.new_empty(shape, dtype=dtype)

@@ -59,8 +59,8 @@ class QuantizedRaggedPageAttention:
             raise ValueError(f"{logits_soft_cap=} must not be 0.0.")
         if queries.requires_grad or kv_scales.requires_grad:
             raise NotImplementedError("quantized_ragged_page_attention is forward-only; detach the inputs")
-        index = _on_device("quantized_ragged_page_attention", queries, kv_cache=kv_cache, kv_scales=kv_scales, context_lens=context_lens,
-                           block_tables=block_tables, query_start_loc=query_start_loc, num_seqs=num_seqs)
+        index = _on_device("quantized_ragged_page_attention", ("queries", queries), ("kv_cache", kv_cache), ("kv_scales", kv_scales),
+                           ("context_lens", context_lens), ("block_tables", block_tables), ("query_start_loc", query_start_loc), ("num_seqs", num_seqs))
         if _current_device() != index:
             with torch.cuda.device(index):
                 return self.run(queries, kv_cache, kv_scales, context_lens, block_tables, query_start_loc, num_seqs, softmax_aux,
@@ -68,7 +68,7 @@ class QuantizedRaggedPageAttention:
         out = queries.new_empty(shape)
         if total_tokens == 0:
             return out
-        queries, token_stride, head_stride = _rows(queries)
+        queries, address, token_stride, head_stride = _rows(queries, shape)
         context_lens, block_tables, query_start_loc = context_lens.contiguous(), block_tables.contiguous(), query_start_loc.contiguous()
         sinks = None
         if softmax_aux is not None and softmax_aux.shape[-1] > 0:
@@ -77,7 +77,7 @@ class QuantizedRaggedPageAttention:
         if size is None:
             size = self._workspace_bytes(index, dtype, head_dim)
         workspace = _call_workspace(queries.device, size, _raw_stream(index))
-        _call(self._entry, index, queries.data_ptr(), kv_cache.data_ptr(), kv_scales.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(),
+        _call(self._entry, index, address, kv_cache.data_ptr(), kv_scales.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(),
               query_start_loc.data_ptr(), num_seqs.data_ptr(), 0 if sinks is None else sinks.data_ptr(), out.data_ptr(),
               workspace.data_ptr(), workspace.numel(), token_stride, head_stride, total_tokens, num_q_heads, num_kv_heads, head_dim, page_size, block,
               num_pages, max_num_seqs, pages_per_seq, 0 if sinks is None else sinks.shape[1],
