@@ -134,7 +134,8 @@ struct FewLds {
   int start[kN + 1], cached[kN], from[kN];  // cached: -1 where the request's tokens do not run
 };
 
-template <int kN>
+// kPer: requests that a thread keeps in registers, all loaded at once; 0: as many as there are, loaded for every pass.
+template <int kN, int kPer>
 __global__ __launch_bounds__(kN) void block_tables_plan_kernel(RpaBlockTablesParams p, int write_entries) {
   constexpr int kWaves = kN / 64;
   __shared__ Pair lds[3][kWaves];
@@ -145,30 +146,37 @@ __global__ __launch_bounds__(kN) void block_tables_plan_kernel(RpaBlockTablesPar
   const int n = clipped_count(p);
   const int2 ring = ring_state(p);
   Move* moves = reinterpret_cast<Move*>(p.scratch);
-  const Request only = request(p, n, min(s0, n_all - 1));
-  const auto get = [&](int s) { return per == 1 ? only : request(p, n, s); };
+  Request kept[kPer > 0 ? kPer : 1];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) kept[k] = request(p, n, min(s0 + k, n_all - 1));
+  const auto each = [&](auto&& f) {
+    if constexpr (kPer > 0) {
+#pragma unroll
+      for (int k = 0; k < kPer; ++k)
+        if (s0 + k < s1) f(s0 + k, kept[k]);
+    } else {
+      for (int s = s0; s < s1; ++s) f(s, request(p, n, s));
+    }
+  };
 
   Pair sum = {0, 0}, total;
-  for (int s = s0; s < s1; ++s) {
-    const Request r = get(s);
+  each([&](int, const Request& r) {
     sum.a += max(r.q, 0);
     sum.b += r.q < 0 ? r.have : 0;
-  }
+  });
   const Pair at = block_prefix<kWaves>(sum, lds[0], &total);  // first token and first page given back of this thread's requests
   sum = {0, 0};
   int64_t end = at.a;
-  for (int s = s0; s < s1; ++s) {
-    const Request r = get(s);
+  each([&](int, const Request& r) {
     end += max(r.q, 0);
     sum.a += fits(p, r, end) ? need_of(p, r) : 0;
-  }
+  });
   const Pair taken = block_prefix<kWaves>(sum, lds[1], &total);
   Pair last = {0, 0};  // behind the last page taken and given back: whoever does not fit, nobody behind it does
   int64_t start = at.a, back = at.b, need = taken.a;
   Move m = {0, 0, 0, 0};
   int first_token = 0, cached = -1;
-  for (int s = s0; s < s1; ++s) {
-    const Request r = get(s);
+  each([&](int s, const Request& r) {
     end = start + max(r.q, 0);
     const bool ok = fits(p, r, end);
     const int want = ok ? need_of(p, r) : 0, gives = r.q < 0 ? r.have : 0;
@@ -190,7 +198,7 @@ __global__ __launch_bounds__(kN) void block_tables_plan_kernel(RpaBlockTablesPar
     back += gives;
     if (m.taken > 0) last.a = need;
     if (m.given > 0) last.b = back;
-  }
+  });
   const int behind_last = static_cast<int>(min(start, static_cast<int64_t>(p.total_tokens)));
   if (s0 < n_all && s1 == n_all) p.query_start_loc[n_all] = behind_last;
 #pragma unroll
@@ -214,7 +222,7 @@ __global__ __launch_bounds__(kN) void block_tables_plan_kernel(RpaBlockTablesPar
     p.free_state_out[1] = static_cast<int>(ring.y - last.a + last.b);
   }
   if (!write_entries) return;  // else: a thread has one request at most
-  const int have = only.have;
+  const int have = kept[0].have;
   // Pages: one for most requests of a decode step, which its thread moves; longer moves by the wavefront, one after another.
   if (m.taken == 1) p.block_tables[static_cast<size_t>(s) * p.pages_per_seq + have] = p.free_pages[m.from];
   for (uint64_t long_moves = __ballot(m.taken > 1 || m.given > 0); long_moves != 0; long_moves &= long_moves - 1) {
@@ -256,8 +264,10 @@ int launch_block_tables(const RpaBlockTablesParams& p, hipStream_t stream) {
   // one request and a few tokens.
   const bool few = p.max_num_seqs <= kThreads && p.total_tokens <= 4 * kThreads;
   const bool fewer = p.max_num_seqs <= kFewThreads && p.total_tokens <= 4 * kFewThreads;
-  if (fewer) hipLaunchKernelGGL(block_tables_plan_kernel<kFewThreads>, dim3(1), dim3(kFewThreads), 0, stream, p, 1);
-  else hipLaunchKernelGGL(block_tables_plan_kernel<kThreads>, dim3(1), dim3(kThreads), 0, stream, p, few ? 1 : 0);
+  if (fewer) hipLaunchKernelGGL((block_tables_plan_kernel<kFewThreads, 1>), dim3(1), dim3(kFewThreads), 0, stream, p, 1);
+  else if (p.max_num_seqs <= kThreads) hipLaunchKernelGGL((block_tables_plan_kernel<kThreads, 1>), dim3(1), dim3(kThreads), 0, stream, p, few ? 1 : 0);
+  else if (p.max_num_seqs <= 4 * kThreads) hipLaunchKernelGGL((block_tables_plan_kernel<kThreads, 4>), dim3(1), dim3(kThreads), 0, stream, p, 0);
+  else hipLaunchKernelGGL((block_tables_plan_kernel<kThreads, 0>), dim3(1), dim3(kThreads), 0, stream, p, 0);
   if (hipGetLastError() != hipSuccess) return RPA_ERR_LAUNCH;
   if (few) return RPA_OK;
   const int token_groups = (p.total_tokens + 255) / 256, seq_groups = (p.max_num_seqs + 3) / 4;
