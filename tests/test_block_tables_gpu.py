@@ -152,3 +152,13 @@ def test_serving_steps(kind, captured):
         check_attention(out, x[:, : heads * group].cpu(), ref["codes"], ref["scales"], np.array(want["context_lens"]), want["tables"], starts, n, kind)
         ref.update(tables=want["tables"], ring=want["ring"], cached=np.array(want["cached_lens"]), state=want["free_state"])
     assert refused, "the plan is meant to run out of pages at least once"
+
+
+@pytest.mark.parametrize("n", [1025, 2048, 4096, 4097, 9000])
+@pytest.mark.parametrize("idle", [slice(0, 700), slice(100, 1000), slice(300, None)])
+def test_many_requests_with_long_idle_stretches(n, idle):
+    """Tokens whose request lies far behind the previous token's, and requests of several threads' share."""
+    rng = np.random.default_rng(n)
+    q, cached, tables, ring, state = scene(rng, n, 16, 100, 40, spare=2 * n)
+    q[idle] = 0
+    check(q, cached, tables, ring, state, n, 16, int(np.maximum(q, 0).sum()) + 300)
