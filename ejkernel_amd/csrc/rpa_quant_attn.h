@@ -23,7 +23,7 @@
 //
 // What bounds it, on a device that copies at 4.9 TB/s, reads at 6.2 TB/s and multiplies bf16 matrices at 1325 TFLOP/s:
 //   - decode, 256 sequences of up to 8192 keys, 32/8 heads of 128: the reads, 2.3 GB in 413 us = 5.6 TB/s;
-//   - decode behind a window of 4096 (64 x 4 tokens, 16/8 heads of 256): the reads, 174 us = 4.8 TB/s;
+//   - decode behind a window of 4096 (64 x 4 tokens, 16/8 heads of 256): the reads, 172 us = 4.9 TB/s;
 //   - chunks: instruction issue.  A 32-key step of a 48-row wavefront at head_dim 128 is 48 matrix instructions of 16
 //     cycles and about 300 vector instructions -- 80 to widen the codes (e4m3; 210 for int8), 60 for each 16 rows' softmax,
 //     eight of them exponentials of four times the cost -- so that vector instructions issue in 61 % of all cycles, the matrix
@@ -1069,11 +1069,13 @@ __global__ __launch_bounds__(256, 2) void quant_attention_kernel(QuantArgs) {
   // 15.8 us in four, 18.8 us in one).
   const int64_t items = static_cast<int64_t>(seqs_all) * a.p.num_kv_heads;
   int parts = 0, piece = 0;
-  if (items > 0 && items <= a.grid / 2) {
-    parts = max(min(a.grid / 2 / static_cast<int>(items), longest / kThinLeast), 1);
+  // Nearly as many items as workgroups are whole as well (64 x 4 tokens of 8 heads behind a window: 176 us cut evenly, 171 us so).
+  const int places = items <= a.grid / 2 ? a.grid / 2 : a.grid;
+  if (items > 0 && items <= places && (places < a.grid || items * 10 >= a.grid * 9)) {
+    parts = max(min(places / static_cast<int>(items), longest / kThinLeast), 1);
     if (longest - longest / parts < kThinMeet) parts = 1;
     piece = max(((longest - 1) / parts + kThinStep) & -kThinStep, kThinStep);  // parts * piece >= longest
-    if (piece > total[0] / (a.grid / 2) + kThinUneven) parts = 0;
+    if (piece > total[0] / places + kThinUneven) parts = 0;
   }
   const int fixed = parts * piece;
   if (fixed > 0) {

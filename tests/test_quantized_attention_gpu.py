@@ -181,3 +181,10 @@ def test_malformed_device_metadata_stays_in_bounds():
         assert all(torch.equal(x.view(torch.uint8) if x.dtype.itemsize == 1 else x.nan_to_num(), y.view(torch.uint8) if y.dtype.itemsize == 1 else y.nan_to_num())
                    for x, y in zip(before, args[1:]))
     b.check(quantized_ragged_page_attention(*b.args(), **b.kwargs()))
+
+
+@pytest.mark.parametrize("seqs,heads", [(60, 8), (64, 8), (65, 8), (32, 8), (33, 8), (29, 16), (256, 2), (512, 1), (3, 2)])
+def test_items_as_many_as_workgroups(seqs, heads):
+    """Around half and the whole of the workgroups that 256 compute units take: whole items, equal parts, cuts anywhere."""
+    for lens in ([500] * seqs, [40 + 13 * k % 700 for k in range(seqs)], [3000] + [30] * (seqs - 1)):
+        run(Batch([(1, n) for n in lens], q_heads=heads, kv_heads=heads, dim=16, page=64, block=16, kind="int8", seed=seqs))
