@@ -188,3 +188,30 @@ def test_items_as_many_as_workgroups(seqs, heads):
     """Around half and the whole of the workgroups that 256 compute units take: whole items, equal parts, cuts anywhere."""
     for lens in ([500] * seqs, [40 + 13 * k % 700 for k in range(seqs)], [3000] + [30] * (seqs - 1)):
         run(Batch([(1, n) for n in lens], q_heads=heads, kv_heads=heads, dim=16, page=64, block=16, kind="int8", seed=seqs))
+
+
+def test_two_threads_on_streams_of_their_own():
+    import threading
+
+    batches = [Batch([(1, 3000), (50, 700), (1, 5)], q_heads=8, kv_heads=2, dim=64, page=16, block=16, kind="int8", seed=1),
+               Batch([(1, 900)] * 20 + [(200, 200)], q_heads=8, kv_heads=2, dim=128, page=16, block=16, kind="e4m3", seed=2)]
+    args = [b.args() for b in batches]
+    want = [run(b) for b in batches]
+    same, errors = [[], []], []
+
+    def work(k):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(25):
+                    same[k].append(torch.equal(quantized_ragged_page_attention(*args[k], **batches[k].kwargs()), want[k]))
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(k,)) for k in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and all(len(s) == 25 and all(s) for s in same), errors
