@@ -153,8 +153,9 @@ __device__ __forceinline__ Seq load_seq(Args& a, int n, int s) {
 // part, two workgroups share a compute unit, and the one that was there first gets the larger part of its issue slots and
 // of its memory requests: with equal runs it ends at three quarters of the other's time.  So it gets the longer run: kFirst of
 // kPairUnits, the other the rest (2 x 8192 tokens: 746 us at 64, 724 at 72, 707 at 80; 16 chunks of 512 after 4096: 260, 255
-// and 256; decode steps of 64 x 4 tokens behind a window 173, 173 and 169, of 256 up to 8192 keys alike).  The workgroups of an XCD hold `block` neighbouring runs, those of the first
-// workgroups in front or, where `back` is set, behind.
+// and 256; decode steps of 64 x 4 tokens behind a window 173, 173 and 169, of 256 up to 8192 keys alike).  The workgroups of
+// an XCD hold `block` neighbouring runs; those of its first workgroups lie in front in the first stream and behind in the second,
+// which is dealt out from the grid's back.
 constexpr int kPairUnits = 128, kFirst = 78;
 // x / y of numbers that are not negative: 32 bits nearly always; the rest bit by bit, since the code on the way to the
 // first load is fetched anew by every launch and a 64-bit division is long.
