@@ -301,10 +301,11 @@ __device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
 
 __device__ __forceinline__ f32x4_t mfma(bf16x8_t a, bf16x8_t b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-// A product under its scale: capped in units of log2, or just scaled.
-template <bool kCap>
+// A product under its scale: capped in units of log2, or just scaled.  The quick tanh is off by 1e-7 of the cap, nothing beside
+// probabilities that are rounded to bf16; with fp32 queries the library's is taken, to a unit of its own size.
+template <bool kCap, bool kExact>
 __device__ __forceinline__ float scaled(float s, float c, float cap, float inv_cap) {
-  if constexpr (kCap) return cap * tanh_fast(s * c * inv_cap);
+  if constexpr (kCap) return cap * (kExact ? tanhf(s * c * inv_cap) : tanh_fast(s * c * inv_cap));
   return s * c;
 }
 
@@ -549,7 +550,7 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float x = scaled<kCap>(sa[mt][u][r], c[u], cap2, inv_cap);
+            const float x = scaled<kCap, kParts == 3>(sa[mt][u][r], c[u], cap2, inv_cap);
             sa[mt][u][r] = !edge || (k + r < hi[mt] && k + r >= hi[mt] - window) ? x : -INFINITY;
           }
         c[u] = 1.f;

@@ -215,3 +215,25 @@ def test_two_threads_on_streams_of_their_own():
     for t in threads:
         t.join()
     assert not errors and all(len(s) == 25 and all(s) for s in same), errors
+
+
+def test_soft_cap_in_fp32_keeps_fp32_logits():
+    """Two keys, the first of logit 0, whose log-odds give the second's capped logit back.
+
+    It takes nine roundings of its own size (the products' sum, scales, 1 / cap and its product, tanh, cap), each off by 2**-24 / sqrt(3) in
+    the mean square: 4.5 * 3 * 2**-24 / sqrt(3) = 4.7e-7 at most.  The exponential's argument adds 1.5e-7, its value and the
+    output's division and rounding 1e-7: 5.1e-7 in all.  A tanh that is off by 6e-8 of the cap would add 1.3e-6.
+    """
+    rng = np.random.default_rng(0)
+    seqs, heads, dim, cap = 1024, 4, 16, 30.0
+    codes = np.zeros((1, 2 * heads, 16, dim), np.int8)
+    codes[0, 0::2, 1, 3] = 1
+    codes[0, 1::2, 1, :] = 1
+    x = torch.zeros((seqs, heads, dim))
+    x[:, :, 3] = torch.from_numpy(-cap * rng.uniform(0.0625, 0.15, size=(seqs, heads))).float()
+    out = quantized_ragged_page_attention(x.to("cuda:0"), torch.from_numpy(codes).to("cuda:0"), torch.ones((1, 2 * heads, 1), device="cuda:0"),
+                                          torch.full((seqs,), 2, dtype=torch.int32, device="cuda:0"), torch.zeros((seqs, 1), dtype=torch.int32, device="cuda:0"),
+                                          torch.arange(seqs + 1, dtype=torch.int32, device="cuda:0"), seqs, softmax_scale=1.0, logits_soft_cap=cap)
+    p = out[:, :, 5].double().cpu().numpy()
+    off = np.log(p / (1 - p)) - cap * np.tanh(x[:, :, 3].double().numpy() / cap)
+    assert np.sqrt((off**2).mean()) < 7.5e-7
