@@ -3,7 +3,8 @@
 //   out[row] = sum_k p_k v_k vs_k / (sum_k p_k + sum_j e^(sink_j)),  p_k = exp(cap(scale q . k_k ks_k))
 //
 // Codes are widened to bf16, which holds all of them exactly, and multiplied on the matrix units; the scale of a key
-// enters its logit and the scale of a value its probability, in fp32.  With bf16 queries p vs is rounded to bf16 once;
+// enters its logit and the scale of a value its probability, in fp32.  With bf16 queries p vs is two bf16 parts in
+// decode rows and rounded to bf16 once in tiles of rows;
 // with fp32 queries the operands that have 24 bits -- q and p vs -- are split into three bf16 parts each (8 + 8 + 8 bits),
 // three products in place of one, and nothing is rounded below fp32.
 //
@@ -409,6 +410,9 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
                                      const int (&hi)[MT], const Range& range, int full_lo, int full_hi, int k_begin, int k_end, int stride,
                                      RowState<MT, D>& st) {
   constexpr int NP = D / 64, NV = D / 64, NO = D / 16;
+  // Bf16 parts of the probabilities.  The first stream waits for memory, so that with bf16 queries a second part costs it nothing and
+  // leaves the result's own rounding alone.
+  constexpr int kWeightParts = kParts == 1 && MT == 1 ? 2 : kParts;
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, dim = a.p.head_dim;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
@@ -567,7 +571,7 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
     }
     // Probabilities under the running maximum as it stands.  Where some of them are so large that a logit must have passed it
     // by far (or there was none yet), it follows, which happens a few times in a row's walk: no maximum is taken in the others.
-    bf16x8_t pf[MT][kParts];
+    bf16x8_t pf[MT][kWeightParts];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       float pv[8], sum;
@@ -593,7 +597,7 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
       st.l[mt] += sum;
 #pragma unroll
       for (int e = 0; e < 8; ++e) pv[e] *= w[e >> 2];
-      split<kParts>(pv, pf[mt]);
+      split<kWeightParts>(pv, pf[mt]);
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -609,7 +613,7 @@ __device__ __forceinline__ void walk(Args& a, const Seq& q, int s, int h, const 
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int sp = 0; sp < kParts; ++sp) st.acc[mt][4 * j + b] = mfma(v, pf[mt][sp], st.acc[mt][4 * j + b]);
+          for (int sp = 0; sp < kWeightParts; ++sp) st.acc[mt][4 * j + b] = mfma(v, pf[mt][sp], st.acc[mt][4 * j + b]);
       }
     }
     in_order();

@@ -4,7 +4,8 @@ Takes the batch of ``ragged_page_attention`` -- flat queries, context lengths, b
 starts -- and the cache of ``quantized_cache_update``.  Nothing like it is in the reference, whose
 8-bit caches have one scale per tensor and round probabilities to the cache's type: here codes are
 widened, scales enter the logits and the probabilities in float32, and only the products of
-probability and value scale are rounded, to bfloat16 (with float32 queries not even those).
+probability and value scale are rounded: to 16 bits in decode steps, to bfloat16 in longer chunks, with
+float32 queries not at all.
 """
 
 from __future__ import annotations

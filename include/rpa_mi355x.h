@@ -295,7 +295,8 @@ int rpa_ragged_decode_launch(const RpaRaggedDecodeParams* params, void* hip_stre
 
 /* Attention over that cache: queries of every sequence against its keys, causal from the end of its context, with the
  * window, soft cap and sinks of rpa_fwd_launch.  Logits, softmax and sums are fp32; with bf16 queries the probabilities
- * times the value scale are rounded to bf16 for the matrix unit, with fp32 queries nothing is rounded below fp32.
+ * times the value scale are rounded for the matrix unit, to bf16 where a sequence has more than 16 query rows per kv head, to
+ * 16 bits elsewhere; with fp32 queries nothing is rounded below fp32.
  * Rows without a visible key, and rows at or beyond query_start_loc[num_seqs], are zeros. */
 typedef struct RpaQuantParams {
   const void* queries;            /* [total_tokens, num_q_heads, head_dim] bf16 or fp32, strides below; 16-byte aligned */
